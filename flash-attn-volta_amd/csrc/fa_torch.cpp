@@ -1,4 +1,5 @@
-// Autograd nodes of flash_attn / flash_attn_gqa and apply_rotary_qk in C++
+// Autograd nodes of flash_attn / flash_attn_gqa, apply_rotary_qk and
+// apply_rotary_positions in C++
 // (Python module flash_attn_volta._fa_torch), a client of the C ABI in
 // fa_mi355x.h.
 //
@@ -14,6 +15,7 @@
 #include <torch/extension.h>
 
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
 #include <c10/hip/HIPStream.h>
 
 #include <algorithm>
@@ -36,6 +38,7 @@ extern "C" {
 __attribute__((weak)) decltype(fa_rope_qk_fwd) fa_rope_qk_fwd;
 __attribute__((weak)) decltype(fa_rope_qk_bwd) fa_rope_qk_bwd;
 __attribute__((weak)) decltype(fa_rope_qk_workspace_bytes) fa_rope_qk_workspace_bytes;
+__attribute__((weak)) decltype(fa_rotary) fa_rotary;
 }
 
 namespace {
@@ -380,6 +383,94 @@ std::optional<std::tuple<Tensor, Tensor>> rope(const Tensor &q, const Tensor &k,
   return std::make_tuple(r[0], r[1]);
 }
 
+// The rotation by positions (rotary.py's apply_rotary_positions) and, with
+// FA_ROTARY_INVERSE, its gradient: each is the other's.
+struct RotaryFn : public torch::autograd::Function<RotaryFn> {
+  static variable_list rotate(const Tensor &q, const OptTensor &k, const Tensor &positions,
+                              const Tensor &steps, double factor, int64_t dim, int64_t flags) {
+    const c10::DeviceGuard guard(q.device());
+    const bool two = k && k->defined();
+    int64_t st[4][4] = {}, ps[2] = {positions.size(0) == 1 ? 0 : positions.stride(0),
+                                    positions.stride(1)};
+    const Tensor x = kernel_ready(q, st[0]);
+    Tensor y = two ? kernel_ready(*k, st[1]) : Tensor();
+    variable_list out = {at::empty(q.sizes(), q.options())};
+    kernel_strides(out[0], st[2]);
+    if (two) {
+      out.push_back(at::empty(k->sizes(), k->options()));
+      kernel_strides(out[1], st[3]);
+    }
+    if (positions.scalar_type() == at::kLong) flags |= FA_ROTARY_POS64;
+    check(fa_rotary(x.data_ptr(), two ? y.data_ptr() : nullptr, out[0].data_ptr(),
+                    two ? out[1].data_ptr() : nullptr, steps.data_ptr<int64_t>(), factor, (int)dim,
+                    (int)flags, positions.data_ptr(), ps, (int)q.size(0), (int)q.size(1),
+                    (int)q.size(2), two ? (int)k->size(2) : 0, (int)q.size(3), st[0], st[1], st[2],
+                    st[3], dtype_of(q), stream_of(q)),
+          "fa_rotary");
+    return out;
+  }
+
+  static variable_list forward(AutogradContext *ctx, const Tensor &q, const OptTensor &k,
+                               const Tensor &positions, const Tensor &steps, double factor,
+                               int64_t dim, int64_t flags) {
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({positions, steps});
+    ctx->saved_data["factor"] = factor;
+    ctx->saved_data["dim"] = dim;
+    ctx->saved_data["flags"] = flags;
+    ctx->saved_data["rows"] = positions.size(0);
+    ctx->saved_data["wide"] = positions.scalar_type() == at::kLong;
+    return rotate(q, k, positions, steps, factor, dim, flags);
+  }
+
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    const variable_list s = ctx->get_saved_variables();
+    const int64_t dim = ctx->saved_data["dim"].toInt();
+    const int64_t flags = ctx->saved_data["flags"].toInt() ^ FA_ROTARY_INVERSE;
+    const double factor = ctx->saved_data["factor"].toDouble();
+    variable_list g, d(7);
+    int side[2];
+    for (size_t i = 0; i < grads.size(); ++i)   // a side that needs no gradient is not rotated
+      if (grads[i].defined() && ctx->needs_input_grad(i)) {
+        side[g.size()] = (int)i;
+        g.push_back(grads[i]);
+      }
+    if (g.empty()) return d;
+    check_saved(s[0], {ctx->saved_data["rows"].toInt(), g[0].size(1)},
+                ctx->saved_data["wide"].toBool() ? at::kLong : at::kInt, g[0].device());
+    check_saved(s[1], {dim / 2}, at::kLong, g[0].device());
+    const Tensor steps = s[1].contiguous();
+    const OptTensor second = g.size() > 1 ? OptTensor(g[1]) : OptTensor();
+    const variable_list r =
+        at::GradMode::is_enabled()
+            ? RotaryFn::apply(g[0], second, s[0], steps, factor, dim, flags)
+            : rotate(g[0], second, s[0], steps, factor, dim, flags);
+    for (size_t i = 0; i < g.size(); ++i) d[side[i]] = r[i];
+    return d;
+  }
+};
+
+// (q_out, k_out or None) of arguments that rotary.py has checked, none empty.
+std::tuple<Tensor, OptTensor> rotary(const Tensor &q, const OptTensor &k, const Tensor &positions,
+                                     const Tensor &steps, double factor, int64_t dim,
+                                     int64_t flags) {
+  variable_list r = RotaryFn::apply(q, k, positions, steps, factor, dim, flags);
+  return {r[0], r.size() > 1 ? OptTensor(r[1]) : OptTensor()};
+}
+
+// Whether leaf `t` has a gradient accumulator that was made on another stream
+// than the current one: an autograd graph of it lives there.  The engine makes
+// that stream wait for a backward pass that reaches the leaf, which draws it
+// into the capture of a pass that is being captured, and ending a capture with
+// a stream not joined again ends the process.
+bool held_on_another_stream(const Tensor &t) {
+  if (!t.requires_grad() || !t.is_leaf()) return false;
+  const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+  if (!node) return false;
+  const auto made = node->stream();
+  return made && *made != c10::impl::VirtualGuardImpl(t.device().type()).getStream(t.device());
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_fa_torch, m) {
@@ -395,9 +486,13 @@ PYBIND11_MODULE(_fa_torch, m) {
                  (int)FA_ABI_VERSION, (int)fa_abi_version());
     throw pybind11::error_already_set();
   }
-  m.doc() = "C++ autograd nodes of flash_attn_volta's flash_attn / flash_attn_gqa / apply_rotary_qk";
+  m.doc() = "C++ autograd nodes of flash_attn_volta's flash_attn / flash_attn_gqa / apply_rotary_qk / "
+            "apply_rotary_positions";
   m.def("make_plan", &make_plan, "register a launch plan (ints, sm_scale) -> handle");
   m.def("rope", &rope, "QK-norm + rotary prologue, recording the C++ backward node, or None");
+  m.def("rotary", &rotary, "rotation by positions, recording the C++ backward node");
+  m.def("held_on_another_stream", &held_on_another_stream,
+        "a leaf's gradient accumulator was made on another stream");
   m.def("attn", &attn, "forward of a plan, recording the C++ backward node");
   m.attr("PLAN_INTS") = (int64_t)kPlanInts;
 }

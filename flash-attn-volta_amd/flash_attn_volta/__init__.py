@@ -24,6 +24,12 @@ Beyond the reference (its wrapper requires q, k, v of one shape):
         the attention prologue fused into one pass: optional per-head
         RMSNorm (Qwen3's q_norm / k_norm) and rotary position embedding
         of q and k.
+    RotaryPositions / apply_rotary_positions / rotary_forward / rotary_backward
+        rotary embedding from positions: half or interleaved pairs, part of
+        the head, frequencies scaled for long contexts.
+    PagedKVCache / append_paged / attend_paged / read_paged
+        a paged key/value cache held in 4 bits: appending with the rotation
+        on the way, and the attention over it.
     flash_attn_op
         flash_attn_gqa as torch.library custom ops (flash_attn_volta::fwd,
         flash_attn_volta::bwd) with fake-tensor and autograd registrations,
@@ -37,6 +43,8 @@ from .forward import flash_attn_forward, flash_attn_forward_gqa, flash_attn_volt
 from .backward import flash_attn_backward, flash_attn_backward_gqa
 from .autograd import flash_attn, flash_attn_gqa
 from .rope import apply_rotary_qk, rope_qk_backward, rope_qk_forward
+from .rotary import (RotaryPositions, apply_rotary_positions, rotary_backward, rotary_forward)
+from .paged import PagedKVCache, append_paged, attend_paged, read_paged
 from .ops import flash_attn_op
 from ._runtime import release_workspaces
 
@@ -51,6 +59,14 @@ __all__ = [
     "apply_rotary_qk",
     "rope_qk_forward",
     "rope_qk_backward",
+    "RotaryPositions",
+    "apply_rotary_positions",
+    "rotary_forward",
+    "rotary_backward",
+    "PagedKVCache",
+    "append_paged",
+    "attend_paged",
+    "read_paged",
     "flash_attn_op",
     "release_workspaces",
 ]

@@ -39,6 +39,11 @@ FA_DTYPE_F16 = 0
 FA_DTYPE_BF16 = 1
 FA_HALF_COLS = 0x100
 
+# flags of fa_rotary and fa_paged_append
+FA_ROTARY_INTERLEAVED = 1
+FA_ROTARY_INVERSE = 2
+FA_ROTARY_POS64 = 4
+
 # Every symbol include/fa_mi355x.h declares.
 EXPORTED_SYMBOLS = (
     "fa_abi_version",
@@ -63,6 +68,11 @@ EXPORTED_SYMBOLS = (
     "fa_rope_qk_fwd",
     "fa_rope_qk_workspace_bytes",
     "fa_rope_qk_bwd",
+    "fa_rotary",
+    "fa_paged_append",
+    "fa_paged_read",
+    "fa_paged_attn_workspace_bytes",
+    "fa_paged_attn",
 )
 
 _lock = threading.Lock()
@@ -71,6 +81,12 @@ _lib = None
 _i64x4 = ctypes.POINTER(ctypes.c_int64)
 _vp = ctypes.c_void_p
 _ci = ctypes.c_int
+
+
+class PagedCacheStruct(ctypes.Structure):
+    """fa_paged_cache"""
+    _fields_ = [("k_codes", _vp), ("k_scales", _vp), ("v_codes", _vp), ("v_scales", _vp),
+                ("pages", _ci), ("page_size", _ci), ("heads", _ci), ("width", _ci)]
 
 
 class LibraryNotBuilt(RuntimeError):
@@ -173,6 +189,22 @@ def _declare(lib):
                                    _ci, _ci, _ci, _ci, _ci,
                                    _i64x4, _i64x4, _i64x4, _i64x4, _i64x4, _i64x4,
                                    _i64x2, _ci, _vp]
+    _i64, _f64, _cache = ctypes.c_int64, ctypes.c_double, ctypes.POINTER(PagedCacheStruct)
+    lib.fa_rotary.restype = _ci
+    lib.fa_rotary.argtypes = [_vp, _vp, _vp, _vp, _vp, _f64, _ci, _ci, _vp, _i64x2,
+                              _ci, _ci, _ci, _ci, _ci, _i64x4, _i64x4, _i64x4, _i64x4, _ci, _vp]
+    lib.fa_paged_append.restype = _ci
+    lib.fa_paged_append.argtypes = [_cache, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _f64,
+                                    _ci, _ci, _ci, _ci, _ci, _ci,
+                                    _i64x4, _i64x4, _i64x4, _i64x4, _ci, _vp]
+    lib.fa_paged_read.restype = _ci
+    lib.fa_paged_read.argtypes = [_cache, _vp, _i64, _vp, _vp, _vp, _vp, _ci, _ci, _ci, _ci, _vp]
+    lib.fa_paged_attn_workspace_bytes.restype = ctypes.c_size_t
+    lib.fa_paged_attn_workspace_bytes.argtypes = [_ci, _ci, _ci, _ci, _ci]
+    lib.fa_paged_attn.restype = _ci
+    lib.fa_paged_attn.argtypes = [_vp, _cache, _vp, _i64, _vp, _vp, _vp, _vp, _vp,
+                                  ctypes.c_size_t, _ci, _ci, _ci, _ci, _i64x4, ctypes.c_float,
+                                  _ci, _vp]
 
 
 def load(path: str | None = None):
@@ -192,7 +224,10 @@ def load(path: str | None = None):
         v = lib.fa_abi_version()        # before the symbols that another version may lack
         if v != ABI_VERSION:
             raise LibraryNotBuilt(f"{p} has ABI version {v}, expected {ABI_VERSION}; rebuild it")
-        _declare(lib)
+        try:
+            _declare(lib)
+        except AttributeError as e:     # same version, built before an entry point was added
+            raise LibraryNotBuilt(f"{p}: {e}; rebuild it") from e
         if path is None:
             _lib = lib
         return lib

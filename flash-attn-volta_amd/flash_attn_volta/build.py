@@ -14,23 +14,24 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import tempfile
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG_DIR)                  # flash-attn-volta_amd/
 CSRC = os.path.join(ROOT, "csrc")
-SOURCES = [os.path.join(CSRC, "fa_api.hip")]
+SOURCES = [os.path.join(CSRC, f) for f in ("fa_api.hip", "fa_cache.hip")]
 # The C-ABI header (fa_mi355x.h): the repository's include/ directory, or the
 # directory named by FA_MI355X_INCLUDE when the package is built elsewhere.
 INCLUDE_DIR = os.environ.get("FA_MI355X_INCLUDE",
                              os.path.join(os.path.dirname(ROOT), "include"))
-HEADERS = [os.path.join(CSRC, f) for f in ("fa_common.hpp", "fa_fwd.hpp", "fa_bwd.hpp", "fa_rope.hpp")]
+HEADERS = [os.path.join(CSRC, f) for f in ("fa_common.hpp", "fa_fwd.hpp", "fa_bwd.hpp", "fa_rope.hpp",
+                                             "fa_rotary.hpp", "fa_paged.hpp")]
 OUT = os.path.join(PKG_DIR, "libfa_mi355x.so")
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",
     "-O3",
     "-std=c++17",
-    "-shared",
     "-fPIC",
     "-Wall",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
@@ -52,19 +53,34 @@ def build_library(verbose: bool = True) -> str:
     if not os.path.exists(header):
         raise RuntimeError(f"{header} not found: set FA_MI355X_INCLUDE to the directory "
                            "holding the C-ABI header")
-    cmd = [hipcc()] + HIPCC_FLAGS + ["-I", INCLUDE_DIR] + SOURCES + ["-o", tmp]
-    if verbose:
-        print("[build]", " ".join(cmd), flush=True)
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    # hipcc's host pass warns that it does not know the packed-fp32 feature.
-    noise = "is not a recognized feature for this target"
-    err = "\n".join(l for l in res.stderr.splitlines() if noise not in l)
-    if res.returncode != 0:
-        raise RuntimeError(f"hipcc failed ({res.returncode}):\n{err}")
-    if err.strip() and verbose:
-        print(err, file=sys.stderr)
+    # one object a source, compiled side by side, then linked
+    with tempfile.TemporaryDirectory(prefix="fa_build_") as work:
+        objects = [os.path.join(work, os.path.basename(s) + ".o") for s in SOURCES]
+        jobs = []
+        for src, obj in zip(SOURCES, objects):
+            cmd = [hipcc()] + HIPCC_FLAGS + ["-c", "-I", INCLUDE_DIR, src, "-o", obj]
+            if verbose:
+                print("[build]", " ".join(cmd), flush=True)
+            jobs.append(subprocess.Popen(cmd, stderr=subprocess.PIPE, text=True))
+        for err, job in [(job.communicate()[1], job) for job in jobs]:
+            _check(err, job.returncode, verbose)
+        cmd = [hipcc(), "--offload-arch=gfx950", "-shared", "-fPIC"] + objects + ["-o", tmp]
+        if verbose:
+            print("[build]", " ".join(cmd), flush=True)
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        _check(res.stderr, res.returncode, verbose)
     os.replace(tmp, OUT)
     return OUT
+
+
+def _check(err: str, status: int, verbose: bool) -> None:
+    # hipcc's host pass warns that it does not know the packed-fp32 feature.
+    noise = "is not a recognized feature for this target"
+    err = "\n".join(l for l in err.splitlines() if noise not in l)
+    if status != 0:
+        raise RuntimeError(f"hipcc failed ({status}):\n{err}")
+    if err.strip() and verbose:
+        print(err, file=sys.stderr)
 
 
 TORCH_EXT_SRC = os.path.join(CSRC, "fa_torch.cpp")

@@ -459,6 +459,118 @@ int fa_rope_qk_bwd(const void *dq_out, const void *dk_out, const void *q, const 
                    const int64_t dq_strides[4], const int64_t dk_strides[4],
                    const int64_t cs_strides[2], int dtype, void *stream);
 
+/* Flags of fa_rotary and fa_paged_append. */
+#define FA_ROTARY_INTERLEAVED 1  /* pairs (2j, 2j + 1); else (j, R/2 + j)   */
+#define FA_ROTARY_INVERSE 2      /* negative angles: the gradient            */
+#define FA_ROTARY_POS64 4        /* positions are int64                      */
+
+/*
+ * Rotary position embedding of q and k from positions: in the first
+ * R = rotary_dim columns of each row, pair j (the columns j and R/2 + j, or
+ * 2j and 2j + 1 with FA_ROTARY_INTERLEAVED) is rotated by the row's position
+ * times the pair's frequency,
+ *
+ *   a' = factor (a cos - b sin),  b' = factor (b cos + a sin),
+ *
+ * in fp32, rounded once; the other columns are copied.  steps: (R / 2) int64,
+ * frequency / (2 pi) mod 1 in units of 2^-64, so that position * step in
+ * wrapping 64-bit arithmetic is the angle in turns, without the loss of an
+ * fp32 product at far positions.  positions: int32 (int64 with
+ * FA_ROTARY_POS64), element strides {b, s}; any value, negative ones too.
+ * q, q_out (B, S, H, D); k, k_out (B, S, Hk, D), or Hk = 0 and none.  D a
+ * multiple of 8 up to 256, R even, 2 <= R <= D (else FA_ERR_HEAD_DIM).
+ * FA_ROTARY_INVERSE rotates back: the gradients of q and k from those of
+ * q_out and k_out.
+ *
+ * No counterpart in the reference, which leaves rotary embeddings to
+ * transformers' tables (flash_attn_volta/patch_hf.py:177, :291-303, :462).
+ */
+int fa_rotary(const void *q, const void *k, void *q_out, void *k_out, const int64_t *steps,
+              double factor, int rotary_dim, int flags, const void *positions,
+              const int64_t position_strides[2], int B, int S, int H, int Hk, int D,
+              const int64_t q_strides[4], const int64_t k_strides[4],
+              const int64_t q_out_strides[4], const int64_t k_out_strides[4], int dtype,
+              void *stream);
+
+/*
+ * A paged key/value cache held in 4 bits.  Elements are e2m1 numbers (sign,
+ * 2 exponent bits, 1 mantissa bit: 0, 0.5, 1, 1.5, 2, 3, 4, 6), 32 along D to
+ * a power of two 2^(scale - 127).  N = pages, P = page_size (a power of two,
+ * at least 16), token t of a page, contiguous uint8 tensors:
+ *   k_codes  (N, heads, P, D/2)            byte d / 2, low half: even d
+ *   k_scales (N, heads, P, D/32)
+ *   v_codes  (N, heads, P/4, 16, 4, D/32)  t = 4a + r, d = (D/16) m + j at
+ *                                          [a][m][r][j / 2], low half: even j
+ *   v_scales (N, heads, P/4, D/32, 4)      t = 4a + r at [a][block][r]
+ * Codes 16-byte, scales 4-byte aligned.  The page table of a call is (B,
+ * width) int32: position p of sequence b is slot p % P of page
+ * table[b][p / P].  An id outside [0, pages) is no page: nothing is stored
+ * there and no query sees it.  Scales of 255 are never written; a cache
+ * that holds one has undefined values in that block.
+ */
+typedef struct fa_paged_cache {
+  void *k_codes, *k_scales, *v_codes, *v_scales;
+  int pages, page_size, heads, width;
+} fa_paged_cache;
+
+/*
+ * Stores the keys and values of new tokens: token i < counts[b] (S with
+ * counts NULL; clamped to 0 .. S) of sequence b goes to position start[b] + i.
+ * With `steps` (else NULL) keys are first rotated by that position
+ * (fa_rotary's arguments; in fp64, so that a code is the nearest to the rotated
+ * value itself).  A block's scale is the power of two floor(log2 max|x|) - 2,
+ * a value the nearest e2m1 number (ties to the even code, 6 above).  NaN is
+ * stored as 0, an infinity as the largest finite value of `dtype`; with
+ * FA_DTYPE_F16 the scale is at most 2^13, so that what is held fits fp16.
+ * Positions outside the table store nothing.  Two tokens of a call that name
+ * the same slot leave either's values, or some of each.
+ * q (B, S, H, D), or NULL: every row rotated by its position into q_out (rows
+ * behind counts[b] too).  k, v (B, S, heads, D) in `dtype`.  D in {32, 64, 128}.
+ *
+ * No counterpart in the reference, whose patch leaves the cache to
+ * transformers (flash_attn_volta/patch_hf.py:145-162).
+ */
+int fa_paged_append(const fa_paged_cache *cache, const int32_t *table, int64_t table_stride,
+                    const void *k, const void *v, const void *q, void *q_out,
+                    const int32_t *start, const int32_t *counts, const int64_t *steps,
+                    double factor, int rotary_dim, int flags, int B, int S, int H, int D,
+                    const int64_t k_strides[4], const int64_t v_strides[4],
+                    const int64_t q_strides[4], const int64_t q_out_strides[4], int dtype,
+                    void *stream);
+
+/*
+ * The values held at positions start[b] .. start[b] + n - 1, as contiguous
+ * (B, n, heads, D) tensors of `dtype`; 0 behind counts[b] tokens (NULL: none
+ * is behind) and where no page is.
+ */
+int fa_paged_read(const fa_paged_cache *cache, const int32_t *table, int64_t table_stride, void *k,
+                  void *v, const int32_t *start, const int32_t *counts, int B, int n, int D,
+                  int dtype, void *stream);
+
+/* Bytes of workspace fa_paged_attn needs for these sizes on the current
+ * device (0 for invalid ones).  Independent of the lengths and the cache. */
+size_t fa_paged_attn_workspace_bytes(int B, int Sq, int H, int Hk, int D);
+
+/*
+ * Attention of the newest queries over the cache: sequence b holds
+ * lengths[b] tokens (at most width * P are read), the last counts[b] of them (Sq with counts NULL; clamped to
+ * 0 .. Sq) are those of the queries, and query i sees the positions up to
+ * lengths[b] - counts[b] + i.  A query that sees none, and every query behind
+ * counts[b], gets o = 0 and lse = +inf.  Scores are fp32; keys and values enter
+ * the products as the exact 16-bit values of their codes (fp16: rounded below
+ * 2^-24).  q (B, Sq, H, D), o (B, Sq, H, D) contiguous, lse (B, H, Sq) fp32 or
+ * NULL; query head h reads head h / (H / heads).  The lengths are read on the
+ * device, which shares all sequences' keys out evenly whatever they are.
+ * workspace: fa_paged_attn_workspace_bytes, 16-byte aligned.
+ *
+ * No counterpart in the reference, whose patch falls back to eager attention
+ * with a cache (flash_attn_volta/patch_hf.py:145-162).
+ */
+int fa_paged_attn(const void *q, const fa_paged_cache *cache, const int32_t *table,
+                  int64_t table_stride, const int32_t *lengths, const int32_t *counts, void *o,
+                  float *lse, void *workspace, size_t workspace_bytes, int B, int Sq, int H, int D,
+                  const int64_t q_strides[4], float sm_scale, int dtype, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
