@@ -174,25 +174,30 @@ int launch_read_d(const fa::ReadArgs &a, int D, hipStream_t st) {
 
 // -- attention -------------------------------------------------------------------
 
-// The launch of these sizes: column tiles of 16 rows a workgroup, row tiles,
-// chunks aimed at (for each head and row tile) and at most.
+// The launch of these sizes: the kernel (`nt` column tiles of 16 rows a
+// workgroup, 0: the one for many rows), row tiles, chunks aimed at (for each
+// head and row tile) and at most.
 struct AttnPlan {
   int nt, row_tiles, target, slots;
   int64_t rows;
-  size_t o_bytes(int Hk, int D) const { return (size_t)slots * Hk * rows * D * sizeof(float); }
+  // partial results: none where no sequence is split
+  size_t o_bytes(int Hk, int D) const {
+    return target > 1 ? (size_t)slots * Hk * rows * D * sizeof(float) : 0;
+  }
   size_t bytes(int Hk, int D) const {
-    return o_bytes(Hk, D) + (size_t)slots * Hk * rows * 2 * sizeof(float);
+    return target > 1 ? o_bytes(Hk, D) + (size_t)slots * Hk * rows * 2 * sizeof(float) : 0;
   }
 };
 
 AttnPlan attn_plan(int B, int Sq, int H, int Hk, int cus) {
   AttnPlan p;
   p.rows = (int64_t)Sq * (H / Hk);
-  p.nt = p.rows <= 16 ? 1 : 2;
-  p.row_tiles = (int)((p.rows + 16 * p.nt - 1) / (16 * p.nt));
-  const int64_t want = (int64_t)8 * cus / ((int64_t)Hk * p.row_tiles);
+  p.nt = p.rows <= 16 ? 1 : (p.rows <= 32 ? 2 : 0);
+  const int tile = p.nt ? 16 * p.nt : fa::kRowsTile;
+  p.row_tiles = (int)((p.rows + tile - 1) / tile);
+  const int64_t want = (int64_t)(p.nt ? 8 : 3) * cus / ((int64_t)Hk * p.row_tiles);
   p.target = want < 1 ? 1 : (int)want;
-  p.slots = p.target + B;
+  p.slots = p.target > 1 ? p.target + B : B;
   return p;
 }
 
@@ -209,9 +214,12 @@ int launch_attn(const fa::PagedAttnArgs &a, const AttnPlan &p, hipStream_t st) {
   const dim3 grid((unsigned)(p.slots * a.cache.Hk), (unsigned)p.row_tiles);
   if (p.nt == 1)
     fa::fa_paged_few_kernel<E, D, 1><<<grid, 256, 0, st>>>(a);
-  else
+  else if (p.nt == 2)
     fa::fa_paged_few_kernel<E, D, 2><<<grid, 256, 0, st>>>(a);
+  else
+    fa::fa_paged_rows_kernel<E, D><<<grid, 256, 0, st>>>(a);
   if (int rc = launch_status()) return rc;
+  if (p.target == 1) return FA_OK;
   fa::fa_paged_merge_kernel<E, D>
       <<<dim3((unsigned)p.rows, (unsigned)a.cache.Hk, (unsigned)a.B), 256, 0, st>>>(a);
   return launch_status();
@@ -366,8 +374,10 @@ int fa_paged_attn(const void *q, const fa_paged_cache *cache, const int32_t *tab
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const int Hk = cache->heads;
   const AttnPlan p = attn_plan(B, Sq, H, Hk, stream_cus(st));
-  if (workspace == nullptr || workspace_bytes < p.bytes(Hk, D)) return FA_ERR_WORKSPACE;
-  if (!aligned(workspace, 16)) return FA_ERR_ALIGNMENT;
+  if (p.bytes(Hk, D) > 0) {
+    if (workspace == nullptr || workspace_bytes < p.bytes(Hk, D)) return FA_ERR_WORKSPACE;
+    if (!aligned(workspace, 16)) return FA_ERR_ALIGNMENT;
+  }
   fa::PagedAttnArgs a{};
   a.cache = device_cache(cache, table, table_stride);
   a.q = static_cast<const f16 *>(q);

@@ -317,7 +317,9 @@ __device__ __forceinline__ int wave_sum(int x) {
 // Splits all sequences' keys evenly: chunks of the same whole number of units
 // (the last of a sequence shorter), about `target` of them, whatever the lengths.  The
 // host knows no lengths; every wave counts them for itself (B loads) and finds
-// the sequence of its slot.  slots >= target + B covers every chunk.  With
+// the sequence of its slot; one that holds nothing is a chunk too, which writes
+// its zeros.  target + B slots cover every chunk, B with a target of 1 (then no
+// sequence is split).  With
 // `by_sequence` the argument is a sequence and its chunks are returned.
 __device__ __forceinline__ bool find_chunk(const PagedAttnArgs &a, int want, bool by_sequence,
                                            Chunk &out) {
@@ -333,7 +335,7 @@ __device__ __forceinline__ bool find_chunk(const PagedAttnArgs &a, int want, boo
   for (int b0 = 0; b0 < a.B; b0 += 64) {
     const int b = b0 + lane;
     const int u = b < a.B ? (held_keys(a, b) + kUnit - 1) / kUnit : 0;
-    const int n = (u + units - 1) / units;
+    const int n = b < a.B ? max(1, (u + units - 1) / units) : 0;
     int upto = n;                       // inclusive prefix sum
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) {
@@ -612,9 +614,197 @@ __global__ __launch_bounds__(256) void fa_paged_few_kernel(PagedAttnArgs a) {
   }
 }
 
+// Many query rows (prompt chunks): workgroup (slot x head, row tile of 128 rows),
+// 4 waves of 32 rows.  Bound by arithmetic, half of it not matrix products, so
+// the codes are turned into 16-bit values once a workgroup: wave w converts keys
+// 16w .. 16w + 15 of each 64-key tile into LDS, one tile ahead of the products
+// and with the next tile's codes in flight.  LDS holds both operands as their
+// 16-byte fragments: K as [column chunk of 8][key], V as [4-key pairs][column][8
+// keys], so every fragment is one conflict-free 16-byte read.
+// O^T tile dt, row rr is column (D/16)(rr / 2) + 2 dt + rr % 2: the order in
+// which code bytes give them.
+constexpr int kRowsTile = 128, kRowsKeys = 64;
+
+template <typename E, int D>
+__global__ __launch_bounds__(256, 2) void fa_paged_rows_kernel(PagedAttnArgs a) {
+  constexpr int NS = D / 16, ND = D / 32;
+  __shared__ u32x4 s_k[2][D / 8][kRowsKeys];
+  __shared__ u32x2 s_v[2][kRowsKeys / 8][ND][32][2];   // [16-key part, h][dt][rr][4 keys, +8]
+  __shared__ int s_hole[2][4];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int m = lane & 15, g = lane >> 4;              // as a converter
+  const int n = lane & 31, hf = lane >> 5;             // as an owner of row n
+  const int Hk = a.cache.Hk, hk = blockIdx.x % Hk, slot = blockIdx.x / Hk;
+  Chunk ch;
+  if (!find_chunk(a, slot, false, ch)) return;
+  const int b = ch.b, rows = a.Sq * a.G;
+  const int row0 = (gridDim.y - 1 - blockIdx.y) * kRowsTile;   // the longest sweeps first
+  const int held = held_keys(a, b);
+  const int count = a.counts ? min(max(a.counts[b], 0), a.Sq) : a.Sq;
+  const int base = a.lengths[b] - count;
+
+  const int row = row0 + 32 * w + n, qi = row / a.G;
+  const int h = hk * a.G + (row - qi * a.G);
+  const bool real = row < rows && qi < count;
+  const int last = real ? base + qi : -1;
+  vec8<E> qf[NS];
+  {
+    const f16 *qp = a.q + b * a.qs[0] + (int64_t)(real ? qi : 0) * a.qs[1] +
+                    (real ? h : 0) * a.qs[2] + 8 * hf;
+#pragma unroll
+    for (int t = 0; t < NS; ++t) {
+      u32x4 raw = *reinterpret_cast<const u32x4 *>(qp + 16 * t);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) raw[j] = real ? raw[j] ^ a.flip : 0u;
+      qf[t] = __builtin_bit_cast(vec8<E>, raw);
+    }
+  }
+  const int key0 = ch.index * ch.keys;
+  const int i_first = row0 / a.G, i_last = min((row0 + kRowsTile - 1) / a.G, count - 1);
+  const int end = i_first < count ? min(min(held, key0 + ch.keys), base + i_last + 1) : 0;
+  // this wave's rows see every key below `all` and none from `wend` on
+  const int wi = (row0 + 32 * w) / a.G;
+  const int all = base + wi + 1;
+  const int wend = wi < count ? min(end, base + min((row0 + 32 * w + 31) / a.G, count - 1) + 1) : 0;
+
+  float mx = kLowest, l = 0.0f;
+  floatx16 o[ND];
+#pragma unroll
+  for (int t = 0; t < ND; ++t) o[t] = floatx16{};
+
+  Tile16<D> raw;
+  auto load = [&](int key) { load_tile<D>(a.cache, b, hk, key + 16 * w, end, m, g, raw); };
+  auto convert = [&](int buf) {
+    const float sc = fp4_scale(raw.ks);
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t)
+      s_k[buf][(D / 32) * g + t][16 * w + m] = fp4_row8<E>(raw_word<D>(raw.k, t), sc);
+    float vs[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) vs[r] = fp4_scale((raw.vs >> (8 * r)) & 0xFFu);
+    auto columns = [&](auto S) {
+      constexpr int s = decltype(S)::value;
+      uint32_t x[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[r] = v_pair<E, D, s>(raw.v, r, vs[r]);
+      u32x2 *to = &s_v[buf][2 * w + (g & 1)][s][2 * m][g >> 1];
+      to[0] = u32x2{__builtin_amdgcn_perm(x[1], x[0], 0x05040100u),
+                    __builtin_amdgcn_perm(x[3], x[2], 0x05040100u)};
+      to[2] = u32x2{__builtin_amdgcn_perm(x[1], x[0], 0x07060302u),
+                    __builtin_amdgcn_perm(x[3], x[2], 0x07060302u)};
+    };
+    columns(std::integral_constant<int, 0>{});
+    if constexpr (ND > 1) columns(std::integral_constant<int, 1>{});
+    if constexpr (ND > 2) {
+      columns(std::integral_constant<int, 2>{});
+      columns(std::integral_constant<int, 3>{});
+    }
+    if (lane == 0) s_hole[buf][w] = raw.hole;
+  };
+
+  if (key0 < end) {
+    load(key0);
+    convert(0);
+    if (key0 + kRowsKeys < end) load(key0 + kRowsKeys);
+  }
+  __syncthreads();
+  int buf = 0;
+  for (int key = key0; key < end; key += kRowsKeys) {
+    if (key + kRowsKeys < end) {
+      convert(buf ^ 1);
+      if (key + 2 * kRowsKeys < end) load(key + 2 * kRowsKeys);
+    }
+    if (key < wend) {
+      floatx16 s[2];
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+        s[kt] = floatx16{};
+#pragma unroll
+        for (int t = 0; t < NS; ++t)
+          s[kt] = mfma32(__builtin_bit_cast(vec8<E>, s_k[buf][2 * t + hf][32 * kt + n]), qf[t], s[kt]);
+      }
+      const bool holes = s_hole[buf][0] | s_hole[buf][1] | s_hole[buf][2] | s_hole[buf][3];
+      if (key + kRowsKeys > all || key + kRowsKeys > end || __builtin_amdgcn_readfirstlane(holes)) {
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int kk = key + 32 * kt + c_row(i, hf);
+            if (kk > last || kk >= end || s_hole[buf][2 * kt + i / 8]) s[kt][i] = kNegInf;
+          }
+      }
+      float top = s[0][0];
+#pragma unroll
+      for (int i = 1; i < 32; ++i) top = fmaxf(top, s[i >> 4][i & 15]);
+      top *= a.c;
+      // a new maximum only where the old one is left behind by 2^8
+      if (__any(top > mx + 8.0f)) {
+        const float t = fmaxf(max_xor32(top), mx);
+        const float f = fast_exp2(mx - t);
+        mx = t;
+        l *= f;
+#pragma unroll
+        for (int t2 = 0; t2 < ND; ++t2) o[t2] *= f;
+      }
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          vec8<E> p;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float e = fast_exp2(s[kt][8 * u + i] * a.c - mx);
+            l += e;
+            p[i] = (E)e;
+          }
+#pragma unroll
+          for (int t = 0; t < ND; ++t)
+            o[t] = mfma32(*reinterpret_cast<const vec8<E> *>(&s_v[buf][4 * kt + 2 * u + hf][t][n][0]),
+                          p, o[t]);
+        }
+    }
+    __syncthreads();
+    buf ^= 1;
+  }
+
+  if (row >= rows) return;
+  l += xor32(l);
+  const bool seen = real && l != 0.0f;                  // (NaN counts as seen)
+  const bool whole = ch.count == 1;
+  const float f = whole ? (seen ? 1.0f / l : 0.0f) : (real ? 1.0f : 0.0f);
+  const int64_t part = ((int64_t)slot * Hk + hk) * rows + row;
+  E *out = reinterpret_cast<E *>(a.o) + (((int64_t)b * a.Sq + qi) * a.H + h) * D;
+  // registers 2j, 2j + 1 of every dt are 2 ND consecutive columns
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int d = NS * (c_row(2 * j, hf) / 2);
+    float x[2 * ND];
+#pragma unroll
+    for (int t = 0; t < ND; ++t) {
+      x[2 * t] = seen || !whole ? o[t][2 * j] * f : 0.0f;
+      x[2 * t + 1] = seen || !whole ? o[t][2 * j + 1] * f : 0.0f;
+    }
+    if (whole) {
+      E y[2 * ND];
+#pragma unroll
+      for (int t = 0; t < 2 * ND; ++t) y[t] = (E)x[t];
+      __builtin_memcpy(__builtin_assume_aligned(out + d, 4 * ND), y, sizeof y);
+    } else {
+      __builtin_memcpy(__builtin_assume_aligned(a.part_o + part * D + d, 8 * ND), x, sizeof x);
+    }
+  }
+  if (hf != 0) return;
+  if (!whole) {
+    a.part_ml[part * 2] = mx;
+    a.part_ml[part * 2 + 1] = real ? l : 0.0f;
+  } else if (a.lse) {
+    a.lse[((int64_t)b * a.H + h) * a.Sq + qi] = seen ? (mx + fast_log2(l)) * kLn2 : kPosInf;
+  }
+}
+
 // Joins the chunks of row blockIdx.x of head blockIdx.y of sequence blockIdx.z
-// (rows whose sequence is one chunk were written by its workgroup); a sequence
-// that holds no key gives 0 and an LSE of +inf.
+// (rows whose sequence is one chunk were written by its workgroup).
 template <typename E, int D>
 __global__ __launch_bounds__(256) void fa_paged_merge_kernel(PagedAttnArgs a) {
   const int row = blockIdx.x, hk = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;

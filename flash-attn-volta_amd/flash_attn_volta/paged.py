@@ -326,11 +326,11 @@ def attend_paged(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tensor,
     with _on_device(q.device):
         stream = _stream_ptr(q.device)
         nbytes = _ws_bytes(lib, B, Sq, H, Hk, D)
-        ws = _runtime.workspace(nbytes, q.device, stream)
+        ws = _runtime.workspace(nbytes, q.device, stream) if nbytes else None
         rc = lib.fa_paged_attn(
             q.data_ptr(), cache._struct(page_table.shape[1]), page_table.data_ptr(),
             page_table.stride(0), lengths.data_ptr(), _ptr(counts), out.data_ptr(), _ptr(lse),
-            ws.data_ptr(), nbytes, B, Sq, H, D, kernel_strides(q), float(sm_scale),
+            _ptr(ws), nbytes, B, Sq, H, D, kernel_strides(q), float(sm_scale),
             _DTYPES[cache.dtype], stream)
     _capi.check(rc, "fa_paged_attn")
     return (out, lse) if return_softmax_lse else out

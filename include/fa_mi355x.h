@@ -548,7 +548,8 @@ int fa_paged_read(const fa_paged_cache *cache, const int32_t *table, int64_t tab
                   int dtype, void *stream);
 
 /* Bytes of workspace fa_paged_attn needs for these sizes on the current
- * device (0 for invalid ones).  Independent of the lengths and the cache. */
+ * device (0 where it needs none, or for invalid ones).  Independent of the
+ * lengths and the cache. */
 size_t fa_paged_attn_workspace_bytes(int B, int Sq, int H, int Hk, int D);
 
 /*
@@ -561,7 +562,7 @@ size_t fa_paged_attn_workspace_bytes(int B, int Sq, int H, int Hk, int D);
  * 2^-24).  q (B, Sq, H, D), o (B, Sq, H, D) contiguous, lse (B, H, Sq) fp32 or
  * NULL; query head h reads head h / (H / heads).  The lengths are read on the
  * device, which shares all sequences' keys out evenly whatever they are.
- * workspace: fa_paged_attn_workspace_bytes, 16-byte aligned.
+ * workspace: fa_paged_attn_workspace_bytes, 16-byte aligned (NULL where 0).
  *
  * No counterpart in the reference, whose patch falls back to eager attention
  * with a cache (flash_attn_volta/patch_hf.py:145-162).

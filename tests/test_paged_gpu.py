@@ -5,8 +5,9 @@ read back must equal the oracle's.
 
 attend's tolerance, per output: the final rounding, u |o| with u = eps / 2 of
 the type; each probability's rounding before the second product, 2^-11 (fp16)
-or 2^-16 (two bf16) of sum p |v|, and once more for fp16 below 2^-14, 2^-25 of
-sum |v|; and the scores' errors, which every probability and the sum share in:
+or 2^-16 (two bf16; one, of 8 bits and so 2^-8, with more than 32 rows a
+key/value head, whose kernel is bound by arithmetic) of sum p |v|, and once more
+for fp16 below 2^-14, 2^-25 of sum |v|; and the scores' errors, which every probability and the sum share in:
 a score is off by at most (D + 4) 2^-24 of scale * sum |q k| (fp32 products
 and sums) and its exponential by 2^-21 with the sums' own roundings, all twice,
 of sum p |v|.  lse: the scores' errors, 2^-21 and 2^-23 of itself.
@@ -74,7 +75,9 @@ def _check_attend(out, lse, q, model, table, lengths, counts=None, scale=None):
     ref, ref_lse, abs_out, abs_v, abs_s = orc.attend(_f64(q), model, table, lengths, counts, scale)
     u = torch.finfo(dtype).eps / 2
     e = 2 * ((D + 4) * 2 ** -24 * abs_s + 2 ** -21)
-    up, low = (2 ** -11, 2 ** -25) if dtype == F16 else (2 ** -16, 2 ** -24)
+    many = q.shape[1] * q.shape[2] // model.k.shape[2] > 32
+    up, low = ((2 ** -11, 2 ** -25) if dtype == F16 else
+               (2 ** -8 if many else 2 ** -16, 2 ** -24))
     tol = (u * np.abs(ref) * 1.01 + (up + e.transpose(0, 2, 1)[..., None]) * abs_out + low * abs_v
            + torch.finfo(dtype).tiny * torch.finfo(dtype).eps)
     err = np.abs(_f64(out) - ref)
