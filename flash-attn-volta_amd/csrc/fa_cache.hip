@@ -92,23 +92,31 @@ int check_rotary(const int64_t *steps, double factor, int rotary_dim, int D) {
   return isfinite(factor) ? FA_OK : FA_ERR_SCALE;
 }
 
+int log2_up(int n) {
+  int s = 0;
+  while ((1 << s) < n) ++s;
+  return s;
+}
+
 template <typename E>
-int launch_rotary(const fa::RotaryArgs &a, hipStream_t st) {
+int launch_rotary(fa::RotaryArgs a, int D, hipStream_t st) {
+  a.units = fa::rotary_units(a.rot.r2, a.rot.interleaved, D);
+  a.unit_shift = log2_up(a.units);
   // One token to a workgroup, its heads over several, until the workgroups
   // fill the GPU; then 4, whose angles are one each for the 256 lanes at
   // R = 128.
-  const int64_t chunks = (int64_t)(a.heads[0] + a.heads[1]) * (a.D / 8);
   const int cus = stream_cus(st);
-  const int64_t per_token = (chunks + fa::kRotaryThreads - 1) / fa::kRotaryThreads;
+  const int64_t rows = (int64_t)a.heads[0] + a.heads[1], lanes = fa::kRotaryThreads >> a.unit_shift;
+  const size_t lds = fa::pair_slots(a.rot.r2) * sizeof(fa::CosSin<float>);
   if (a.tokens < 4 * cus) {
-    int64_t y = 2 * cus / a.tokens;
-    if (y > per_token) y = per_token;
-    if (y < 1) y = 1;
-    fa::fa_rotary_kernel<E, 1><<<dim3((unsigned)a.tokens, (unsigned)y), fa::kRotaryThreads,
-                                 a.rot.r2 * sizeof(fa::CosSin<float>), st>>>(a);
+    int64_t y = 4 * cus / a.tokens;
+    const int64_t most = (rows + lanes - 1) / lanes;
+    y = y > most ? most : (y < 1 ? 1 : y);
+    fa::fa_rotary_kernel<E, 1>
+        <<<dim3((unsigned)a.tokens, (unsigned)y), fa::kRotaryThreads, lds, st>>>(a);
   } else {
-    fa::fa_rotary_kernel<E, 4><<<dim3((unsigned)((a.tokens + 3) / 4)), fa::kRotaryThreads,
-                                 4 * a.rot.r2 * sizeof(fa::CosSin<float>), st>>>(a);
+    fa::fa_rotary_kernel<E, 4>
+        <<<dim3((unsigned)((a.tokens + 3) / 4)), fa::kRotaryThreads, 4 * lds, st>>>(a);
   }
   return launch_status();
 }
@@ -145,8 +153,8 @@ fa::PagedCache device_cache(const fa_paged_cache *c, const int32_t *table, int64
 
 template <typename E, int D>
 int launch_append(const fa::AppendArgs &a, dim3 grid, hipStream_t st) {
-  const size_t lds = a.rot.steps ? fa::kAppendTokens * a.rot.r2 *
-                                       (sizeof(fa::CosSin<double>) + sizeof(fa::CosSin<float>))
+  const size_t lds = a.rot.steps ? fa::kAppendTokens * fa::pair_slots(a.rot.r2) *
+                                       sizeof(fa::CosSin<double>)
                                  : 0;
   fa::fa_paged_append_kernel<E, D><<<grid, fa::kAppendThreads, lds, st>>>(a);
   return launch_status();
@@ -277,10 +285,9 @@ int fa_rotary(const void *q, const void *k, void *q_out, void *k_out, const int6
   a.ps = position_strides[1];
   a.pos64 = (flags & FA_ROTARY_POS64) != 0;
   a.S = S;
-  a.D = D;
   a.tokens = tokens;
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  return dtype == FA_DTYPE_F16 ? launch_rotary<f16>(a, st) : launch_rotary<bf16>(a, st);
+  return dtype == FA_DTYPE_F16 ? launch_rotary<f16>(a, D, st) : launch_rotary<bf16>(a, D, st);
 }
 
 int fa_paged_append(const fa_paged_cache *cache, const int32_t *table, int64_t table_stride,
@@ -326,14 +333,22 @@ int fa_paged_append(const fa_paged_cache *cache, const int32_t *table, int64_t t
   a.top = dtype == FA_DTYPE_F16 ? 65504.0f : 3.3895313892515355e38f;
   a.max_byte = dtype == FA_DTYPE_F16 ? 127 + 13 : 127 + 125;
   const int64_t tiles = ((int64_t)S + 14) / 8;
-  // the work of a tile over several workgroups while they do not fill the GPU
+  // Parts of a tile: a lane does up to 4 chunks of keys and values, or units of
+  // q, where the grid fills the GPU without more parts, down to one where not.
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  const int64_t work = ((int64_t)cache->heads + a.H) * (D / 8) * (S < 8 ? S : 8);
-  const int64_t most = (work + fa::kAppendThreads - 1) / fa::kAppendThreads;
-  int64_t y = 2 * stream_cus(st) / (tiles * B);
-  y = y > most ? most : y;
-  y = y < 1 ? 1 : (y > 16 ? 16 : y);
-  const dim3 grid((unsigned)tiles, (unsigned)y, (unsigned)B);
+  const int64_t tok = S < fa::kAppendTokens ? S : fa::kAppendTokens;
+  const int64_t kv = tok * cache->heads * (D / 8);
+  int64_t qu = 0;
+  if (q != nullptr) {
+    a.units = fa::rotary_units(a.rot.r2, a.rot.interleaved, D);
+    a.unit_shift = log2_up(a.units);
+    qu = tok * H << a.unit_shift;
+  }
+  int64_t each = 4 * fa::kAppendThreads;
+  while (each > fa::kAppendThreads && (kv + qu) / each * tiles * B < 8 * stream_cus(st)) each /= 2;
+  auto parts = [&](int64_t n) { return n > 64 * each ? 64 : (n + each - 1) / each; };
+  a.parts = (int)parts(kv);
+  const dim3 grid((unsigned)tiles, (unsigned)(a.parts + parts(qu)), (unsigned)B);
   return dtype == FA_DTYPE_F16 ? launch_append_d<f16>(a, D, grid, st)
                                : launch_append_d<bf16>(a, D, grid, st);
 }

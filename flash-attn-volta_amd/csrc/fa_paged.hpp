@@ -67,7 +67,9 @@ struct AppendArgs {
   int64_t ks[3], vs[3], qs[3], qos[3];   // {b, s, h}
   const int32_t *start, *counts;         // counts: NULL = S everywhere
   RotaryTable rot;                       // steps NULL: no rotation
-  int S, H, tiles;
+  int S, H;
+  int parts;                             // of gridDim.y, those that store keys and values
+  int units, unit_shift;                 // of a row of q (rotary_units)
   float top;                             // largest finite value that is kept
   int max_byte;                          // largest scale byte
 };
@@ -94,8 +96,8 @@ __device__ __forceinline__ uint32_t quantise8(float *y, float top, int max_byte,
     y[i] = y[i] != y[i] ? 0.0f : fminf(fmaxf(y[i], -top), top);
     m = fmaxf(m, fabsf(y[i]));
   }
-  m = fmaxf(m, __shfl_xor(m, 1, 64));
-  m = fmaxf(m, __shfl_xor(m, 2, 64));
+  // (quad_perm [1, 0, 3, 2], then [2, 3, 0, 1]; m >= 0 orders as its bits)
+  m = __uint_as_float(dpp_umax<0x4E, 0xF>(dpp_umax<0xB1, 0xF>(__float_as_uint(m))));
   byte = (unsigned)min(max((int)(__float_as_uint(m) >> 23) - 2, 1), max_byte);
   const float s = fp4_scale(byte);
   uint32_t w = 0;
@@ -107,42 +109,64 @@ __device__ __forceinline__ uint32_t quantise8(float *y, float top, int max_byte,
 }
 
 // Workgroup (tile, part, b): the new tokens at positions 8a .. 8a + 7 of
-// sequence b.  Keys are rotated in fp64, from cosines and sines computed once a
-// token in LDS: a code is the nearest to the rotated value itself, so the same
-// key at the same position gets the same code whichever path computed it.
-// Consecutive lanes are the D/8 chunks of a row, then the tokens, whose 4-byte
-// pieces of an interleaved V group then fill whole lines.  Bound by HBM on
-// prompts and by launch and load latency on single tokens.
+// sequence b; the first parts of a tile store keys and values, the rest rotate q.
+// Keys are rotated in fp64, from cosines and sines computed once a token in LDS: a
+// code is the nearest to the rotated value itself, so the same key at the same
+// position gets the same code whichever path computed it.  q is rotated in
+// fp32, as fa_rotary does.  Consecutive lanes are the D/8 chunks of a key's
+// row, then the tokens, whose 4-byte pieces of an interleaved V group then fill
+// whole lines.  Bound by HBM on prompts and by launch and load latency on single
+// tokens.
 template <typename E, int D>
 __global__ __launch_bounds__(kAppendThreads) void fa_paged_append_kernel(AppendArgs a) {
   extern __shared__ char smem[];
   constexpr int NCH = D / 8;
-  const int r2 = a.rot.steps ? a.rot.r2 : 0;
-  CosSin<double> *cs = reinterpret_cast<CosSin<double> *>(smem);          // [8][R / 2]
-  CosSin<float> *csf = reinterpret_cast<CosSin<float> *>(cs + kAppendTokens * r2);
+  const int r2 = a.rot.steps ? a.rot.r2 : 0, slots = pair_slots(r2);
   const int b = blockIdx.z, tid = threadIdx.x;
   const int64_t start = a.start[b];
-  const int count = a.counts ? min(max(a.counts[b], 0), a.S) : a.S;
-  // tokens i0 .. i0 + nt - 1 of this tile; the rows of q behind the count are
-  // rotated too (they are results, not cache)
+  // tokens i0 .. i0 + nt - 1 of this tile
   const int64_t base = (start & ~(int64_t)(kAppendTokens - 1)) + (int64_t)blockIdx.x * kAppendTokens;
   const int i0 = (int)max((int64_t)0, base - start);
-  const int nt = (int)(min((int64_t)a.S, base + kAppendTokens - start) - i0);
+  int nt = (int)(min((int64_t)a.S, base + kAppendTokens - start) - i0);
+  if ((int)blockIdx.y >= a.parts) {
+    // queries (rows behind the count too: they are results, not cache)
+    if (nt <= 0) return;
+    CosSin<float> *cs = reinterpret_cast<CosSin<float> *>(smem);
+    for (int i = tid; i < nt * r2; i += kAppendThreads) {
+      const int t = i / r2, j = i - t * r2;
+      cs[t * slots + pair_slot(j, r2)] =
+          rotary_cos_sin<float>(start + i0 + t, a.rot.steps[j], (float)a.rot.factor);
+    }
+    if (r2) __syncthreads();
+    const int u = tid & ((1 << a.unit_shift) - 1), lanes = kAppendThreads >> a.unit_shift;
+    if (u >= a.units) return;
+    const int step = lanes * (gridDim.y - a.parts), dt = step / a.H, dh = step - dt * a.H;
+    int t = (blockIdx.y - a.parts) * lanes + (tid >> a.unit_shift), h = t % a.H;
+    t /= a.H;
+    for (; t < nt; t += dt, h += dh) {
+      if (h >= a.H) {
+        h -= a.H;
+        if (++t >= nt) break;
+      }
+      rotate_unit<E>(a.q + b * a.qs[0] + (int64_t)(i0 + t) * a.qs[1] + h * a.qs[2],
+                     a.q_out + b * a.qos[0] + (int64_t)(i0 + t) * a.qos[1] + h * a.qos[2], u,
+                     cs + t * slots, r2, a.rot.interleaved != 0);
+    }
+    return;
+  }
+  if (a.counts) nt = min(nt, a.counts[b] - i0);
   if (nt <= 0) return;
+  CosSin<double> *cs = reinterpret_cast<CosSin<double> *>(smem);
   for (int i = tid; i < nt * r2; i += kAppendThreads) {
     const int t = i / r2, j = i - t * r2;
-    const CosSin<double> v = rotary_cos_sin<double>(start + i0 + t, a.rot.steps[j], a.rot.factor);
-    cs[i] = v;
-    csf[i] = CosSin<float>{(float)v.c, (float)v.s};
+    cs[t * slots + pair_slot(j, r2)] =
+        rotary_cos_sin<double>(start + i0 + t, a.rot.steps[j], a.rot.factor);
   }
   if (r2) __syncthreads();
-  const int Hk = a.cache.Hk, step = gridDim.y * kAppendThreads;
-  const int first = blockIdx.y * kAppendThreads + tid;
-  const int nkv = max(0, min(nt, count - i0));       // tokens to store
-  const int rows = nkv * Hk;
-  // whole blocks of 32 columns stay together: rows * NCH is a multiple of 4
-  for (int i = first; i < rows * NCH; i += step) {
-    const int c = i % NCH, th = i / NCH, h = th / nkv, t = th - h * nkv;
+  const int Hk = a.cache.Hk;
+  // whole blocks of 32 columns stay together: nt * Hk * NCH is a multiple of 4
+  for (int i = blockIdx.y * kAppendThreads + tid; i < nt * Hk * NCH; i += a.parts * kAppendThreads) {
+    const int c = i % NCH, th = i / NCH, h = th / nt, t = th - h * nt;
     const int64_t pos = start + i0 + t;
     const int page = page_of(a.cache, b, pos);
     const int slot = (int)(pos & ((1 << a.cache.page_shift) - 1));
@@ -152,7 +176,7 @@ __global__ __launch_bounds__(kAppendThreads) void fa_paged_append_kernel(AppendA
     load8<E, float>(vr + 8 * c, vy);
     if (r2) {
       double y[8];
-      rotate8<E, double>(kr, c, cs + t * r2, r2, a.rot.interleaved != 0, y);
+      rotate8<E, double>(kr, c, cs + t * slots, r2, a.rot.interleaved != 0, y);
 #pragma unroll
       for (int j = 0; j < 8; ++j) ky[j] = odd_float(y[j]);
     } else {
@@ -181,15 +205,6 @@ __global__ __launch_bounds__(kAppendThreads) void fa_paged_append_kernel(AppendA
       a.cache.k_scales[row * (D / 32) + c / 4] = (uint8_t)kb;
       a.cache.v_scales[(group * (D / 32) + c / 4) * 4 + r] = (uint8_t)vb;
     }
-  }
-  if (a.q == nullptr) return;
-  for (int i = first; i < nt * a.H * NCH; i += step) {
-    const int c = i % NCH, th = i / NCH, t = th / a.H, h = th - t * a.H;
-    const f16 *row = a.q + b * a.qs[0] + (int64_t)(i0 + t) * a.qs[1] + h * a.qs[2];
-    f16 *out = a.q_out + b * a.qos[0] + (int64_t)(i0 + t) * a.qos[1] + h * a.qos[2];
-    float y[8];
-    rotate8<E, float>(row, c, csf + t * r2, r2, a.rot.interleaved != 0, y);
-    store8<E>(out + 8 * c, y);
   }
 }
 

@@ -74,13 +74,18 @@ __device__ __forceinline__ void load8(const f16 *p, F *x) {
   for (int i = 0; i < 8; ++i) x[i] = (F)(float)v[i];
 }
 
-// Columns 8c .. 8c+7 of a row, rotated by the row's table cs[R / 2].  The
-// partner columns of a half-layout chunk are a load of their own (they come
-// from the L1 line that another lane of the wave loads as its own chunk):
-// a lane then owns 8 consecutive columns whatever R is, and groups of lanes
-// own the 32-column blocks that the 4-bit cache shares a scale over.
-// Chunks whose partners are not 8 aligned columns (R % 16) load them one by
-// one; the branch is uniform.
+// Place of pair j in a row's table of cosines and sines in LDS: lanes that own
+// consecutive chunks of 8 columns read consecutive entries.
+__device__ __forceinline__ int pair_slot(int j, int r2) { return (j & 7) * ((r2 + 7) >> 3) + (j >> 3); }
+// Entries of a row's table.
+__host__ __device__ __forceinline__ int pair_slots(int r2) { return 8 * ((r2 + 7) >> 3); }
+
+// Columns 8c .. 8c+7 of a row, rotated by the row's table cs.  The partner
+// columns of a half-layout chunk are a load of their own (they come from the L1
+// line that another lane of the wave loads as its own chunk): a lane then owns 8
+// consecutive columns whatever R is, and groups of 4 lanes own the 32-column
+// blocks that the 4-bit cache shares a scale over.  Chunks whose partners
+// are not 8 aligned columns (R % 16) load them one by one; the branch is uniform.
 template <typename E, typename F>
 __device__ __forceinline__ void rotate8(const f16 *row, int c, const CosSin<F> *cs, int r2,
                                         bool interleaved, F *y) {
@@ -91,7 +96,7 @@ __device__ __forceinline__ void rotate8(const f16 *row, int c, const CosSin<F> *
     for (int j = 0; j < 4; ++j) {
       const int p = 4 * c + j;
       if (p < r2) {
-        const CosSin<F> t = cs[p];
+        const CosSin<F> t = cs[pair_slot(p, r2)];
         y[2 * j] = x[2 * j] * t.c - x[2 * j + 1] * t.s;
         y[2 * j + 1] = x[2 * j + 1] * t.c + x[2 * j] * t.s;
       } else {
@@ -105,10 +110,10 @@ __device__ __forceinline__ void rotate8(const f16 *row, int c, const CosSin<F> *
       const bool low = d < r2;
       F z[8];
       load8<E, F>(row + (low ? d + r2 : d - r2), z);
-      const CosSin<F> *t = cs + (low ? d : d - r2);
+      const CosSin<F> *t = cs + ((low ? d : d - r2) >> 3);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const CosSin<F> v = t[i];
+        const CosSin<F> v = t[i * (r2 >> 3)];
         y[i] = x[i] * v.c + (low ? -z[i] : z[i]) * v.s;
       }
     } else {
@@ -123,7 +128,7 @@ __device__ __forceinline__ void rotate8(const f16 *row, int c, const CosSin<F> *
       if (d < 2 * r2) {
         const bool low = d < r2;
         const F z = (F)(float)*reinterpret_cast<const E *>(row + (low ? d + r2 : d - r2));
-        const CosSin<F> v = cs[low ? d : d - r2];
+        const CosSin<F> v = cs[pair_slot(low ? d : d - r2, r2)];
         y[i] = x[i] * v.c + (low ? -z : z) * v.s;
       }
     }
@@ -138,6 +143,41 @@ __device__ __forceinline__ void store8(f16 *p, const float *y) {
   *reinterpret_cast<vec8<E> *>(p) = v;
 }
 
+// Units of a row, one lane's work each: in the half layout with R % 16 = 0 two
+// chunks of 8 columns that are each other's partners (each is loaded, and its
+// cosines read, once) or one behind R; else one chunk.
+__host__ __device__ __forceinline__ int rotary_units(int r2, bool interleaved, int D) {
+  return !interleaved && (r2 & 7) == 0 ? D / 8 - r2 / 8 : D / 8;
+}
+
+template <typename E>
+__device__ __forceinline__ void rotate_unit(const f16 *row, f16 *out, int u,
+                                            const CosSin<float> *cs, int r2, bool interleaved) {
+  const int pairs = r2 >> 3;
+  if (!interleaved && (r2 & 7) == 0) {
+    if (u < pairs) {
+      float x[8], z[8], y[8];
+      load8<E, float>(row + 8 * u, x);
+      load8<E, float>(row + 8 * u + r2, z);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const CosSin<float> v = cs[u + i * pairs];
+        y[i] = x[i] * v.c - z[i] * v.s;
+        z[i] = z[i] * v.c + x[i] * v.s;
+      }
+      store8<E>(out + 8 * u, y);
+      store8<E>(out + 8 * u + r2, z);
+    } else {
+      const int d = 8 * (u + pairs);
+      *reinterpret_cast<u32x4 *>(out + d) = *reinterpret_cast<const u32x4 *>(row + d);
+    }
+  } else {
+    float y[8];
+    rotate8<E, float>(row, u, cs, r2, interleaved, y);
+    store8<E>(out + 8 * u, y);
+  }
+}
+
 struct RotaryArgs {
   const f16 *x[2];      // q, k
   f16 *y[2];
@@ -148,14 +188,15 @@ struct RotaryArgs {
   const void *positions;
   int64_t pb, ps;       // strides of positions
   int pos64;            // int64 positions
-  int S, D;
+  int S, units, unit_shift;   // units of a row, and log2 of the lanes for them
   int64_t tokens;       // B * S
 };
 
 // One workgroup rotates every head of TOK tokens (or, split over gridDim.y,
 // part of them).  Bound by HBM: each element is read and written once.  The
 // cosines and sines of a token are shared by its heads: computed once per
-// workgroup into LDS, then read by one lane per 8 columns.
+// workgroup into LDS, then read by one lane per unit.  Lanes keep their unit and
+// walk the (token, head) rows, so that the sweep has no division.
 constexpr int kRotaryThreads = 256;
 
 __device__ __forceinline__ int64_t rotary_position(const void *positions, int pos64, int64_t i) {
@@ -166,32 +207,43 @@ __device__ __forceinline__ int64_t rotary_position(const void *positions, int po
 template <typename E, int TOK>
 __global__ __launch_bounds__(kRotaryThreads) void fa_rotary_kernel(RotaryArgs a) {
   extern __shared__ char smem[];
-  CosSin<float> *cs = reinterpret_cast<CosSin<float> *>(smem);   // [TOK][R / 2]
-  const int r2 = a.rot.r2;
+  CosSin<float> *cs = reinterpret_cast<CosSin<float> *>(smem);   // [TOK][pair_slots]
+  __shared__ int64_t s_x[TOK][2], s_y[TOK][2];                   // a token's row offsets
+  const int r2 = a.rot.r2, slots = pair_slots(r2), tid = threadIdx.x;
   const int64_t n0 = (int64_t)blockIdx.x * TOK;
   const int nt = (int)min((int64_t)TOK, a.tokens - n0);
-  for (int i = threadIdx.x; i < nt * r2; i += kRotaryThreads) {
+  if (tid < nt) {
+    const uint32_t n = (uint32_t)(n0 + tid), b = n / (uint32_t)a.S, s = n - b * (uint32_t)a.S;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      s_x[tid][i] = b * a.xs[i][0] + s * a.xs[i][1];
+      s_y[tid][i] = b * a.ys[i][0] + s * a.ys[i][1];
+    }
+  }
+  for (int i = tid; i < nt * r2; i += kRotaryThreads) {
     const int t = i / r2, j = i - t * r2;
     const uint32_t n = (uint32_t)(n0 + t), b = n / (uint32_t)a.S, s = n - b * (uint32_t)a.S;
     const int64_t p = rotary_position(a.positions, a.pos64, b * a.pb + s * a.ps);
     CosSin<float> v = rotary_cos_sin<float>(p, a.rot.steps[j], (float)a.rot.factor);
     if (a.rot.inverse) v.s = -v.s;
-    cs[i] = v;
+    cs[t * slots + pair_slot(j, r2)] = v;
   }
   __syncthreads();
-  const int chunks = a.D / 8, heads = a.heads[0] + a.heads[1];
-  const int work = nt * heads * chunks;
-  for (int i = blockIdx.y * kRotaryThreads + threadIdx.x; i < work;
-       i += gridDim.y * kRotaryThreads) {
-    const int c = i % chunks, th = i / chunks, t = th / heads, hh = th - t * heads;
-    const int side = hh >= a.heads[0];
-    const int h = side ? hh - a.heads[0] : hh;
-    const uint32_t n = (uint32_t)(n0 + t), b = n / (uint32_t)a.S, s = n - b * (uint32_t)a.S;
-    const f16 *row = a.x[side] + b * a.xs[side][0] + s * a.xs[side][1] + h * a.xs[side][2];
-    f16 *out = a.y[side] + b * a.ys[side][0] + s * a.ys[side][1] + h * a.ys[side][2];
-    float y[8];
-    rotate8<E, float>(row, c, cs + t * r2, r2, a.rot.interleaved != 0, y);
-    store8<E>(out + 8 * c, y);
+  const int u = tid & ((1 << a.unit_shift) - 1), lanes = kRotaryThreads >> a.unit_shift;
+  if (u >= a.units) return;
+  const int heads = a.heads[0] + a.heads[1], step = lanes * gridDim.y;
+  const int dt = step / heads, dh = step - dt * heads;
+  int t = (blockIdx.y * lanes + (tid >> a.unit_shift)), hh = t % heads;
+  t /= heads;
+  for (; t < nt; t += dt, hh += dh) {
+    if (hh >= heads) {
+      hh -= heads;
+      if (++t >= nt) break;
+    }
+    const int side = hh >= a.heads[0], h = side ? hh - a.heads[0] : hh;
+    rotate_unit<E>(a.x[side] + s_x[t][side] + h * a.xs[side][2],
+                   a.y[side] + s_y[t][side] + h * a.ys[side][2], u, cs + t * slots, r2,
+                   a.rot.interleaved != 0);
   }
 }
 
