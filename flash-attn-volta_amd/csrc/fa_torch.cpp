@@ -16,6 +16,7 @@
 
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 
 #include <algorithm>
@@ -39,6 +40,10 @@ __attribute__((weak)) decltype(fa_rope_qk_fwd) fa_rope_qk_fwd;
 __attribute__((weak)) decltype(fa_rope_qk_bwd) fa_rope_qk_bwd;
 __attribute__((weak)) decltype(fa_rope_qk_workspace_bytes) fa_rope_qk_workspace_bytes;
 __attribute__((weak)) decltype(fa_rotary) fa_rotary;
+__attribute__((weak)) decltype(fa_paged_append) fa_paged_append;
+__attribute__((weak)) decltype(fa_paged_read) fa_paged_read;
+__attribute__((weak)) decltype(fa_paged_attn) fa_paged_attn;
+__attribute__((weak)) decltype(fa_paged_attn_workspace_bytes) fa_paged_attn_workspace_bytes;
 }
 
 namespace {
@@ -450,14 +455,6 @@ struct RotaryFn : public torch::autograd::Function<RotaryFn> {
   }
 };
 
-// (q_out, k_out or None) of arguments that rotary.py has checked, none empty.
-std::tuple<Tensor, OptTensor> rotary(const Tensor &q, const OptTensor &k, const Tensor &positions,
-                                     const Tensor &steps, double factor, int64_t dim,
-                                     int64_t flags) {
-  variable_list r = RotaryFn::apply(q, k, positions, steps, factor, dim, flags);
-  return {r[0], r.size() > 1 ? OptTensor(r[1]) : OptTensor()};
-}
-
 // Whether leaf `t` has a gradient accumulator that was made on another stream
 // than the current one: an autograd graph of it lives there.  The engine makes
 // that stream wait for a backward pass that reaches the leaf, which draws it
@@ -469,6 +466,158 @@ bool held_on_another_stream(const Tensor &t) {
   if (!node) return false;
   const auto made = node->stream();
   return made && *made != c10::impl::VirtualGuardImpl(t.device().type()).getStream(t.device());
+}
+
+// (q_out, k_out or None) with the node recorded where a gradient is wanted, or
+// None for anything the kernel does not take in place as it is (other dtypes,
+// devices and layouts, empty or misaligned tensors, invalid arguments) and for
+// a capture beside another graph of a leaf: rotary.py's general path copies or
+// raises.  (The host time of a call is most of a decode step's: 13.9 us with the
+// checks in Python.)
+std::optional<std::tuple<Tensor, OptTensor>> rotary(const Tensor &q, const OptTensor &k,
+                                                    const Tensor &positions, const Tensor &steps,
+                                                    double factor, int64_t dim, int64_t flags) {
+  if (q.dim() != 4 || !q.is_cuda() || q.numel() == 0) return std::nullopt;
+  const auto dt = q.scalar_type();
+  const int64_t B = q.size(0), S = q.size(1), D = q.size(3);
+  int64_t st[4];
+  if ((dt != at::kHalf && dt != at::kBFloat16) || D % 8 != 0 || D > 256 || dim > D ||
+      !kernel_strides(q, st) || !aligned(q) || B > INT32_MAX || S > INT32_MAX)
+    return std::nullopt;
+  const bool two = k.has_value();
+  if (two && (k->dim() != 4 || k->numel() == 0 || k->scalar_type() != dt ||
+              k->device() != q.device() || k->size(0) != B || k->size(1) != S ||
+              k->size(3) != D || !kernel_strides(*k, st) || !aligned(*k)))
+    return std::nullopt;
+  const auto pt = positions.scalar_type();
+  if ((pt != at::kInt && pt != at::kLong) || positions.device() != q.device() ||
+      steps.device() != q.device())
+    return std::nullopt;
+  if (positions.dim() < 1 || positions.dim() > 2) return std::nullopt;
+  const Tensor p = positions.dim() == 1 ? positions.unsqueeze(0) : positions;
+  if (p.size(1) != S || (p.size(0) != 1 && p.size(0) != B)) return std::nullopt;
+  variable_list r;
+  if (at::GradMode::is_enabled() && (q.requires_grad() || (two && k->requires_grad()))) {
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None &&
+        (held_on_another_stream(q) || (two && held_on_another_stream(*k))))
+      return std::nullopt;
+    r = RotaryFn::apply(q, k, p, steps, factor, dim, flags);
+  } else {
+    r = RotaryFn::rotate(q, k, p, steps, factor, dim, flags);
+  }
+  return std::make_tuple(r[0], two ? OptTensor(r[1]) : OptTensor());
+}
+
+// The paged cache's calls (paged.py), for arguments that the kernels take in
+// place as they are; None for any others.  `cache` is the address of the
+// fa_paged_cache of the table's width, `like` one of the cache's tensors.
+struct PagedCall {
+  const fa_paged_cache *cache;
+  const Tensor &like;
+  at::ScalarType dtype;
+  int64_t D, B = 0;
+  int code() const { return dtype == at::kHalf ? FA_DTYPE_F16 : FA_DTYPE_BF16; }
+  bool rows(const Tensor &t, int64_t (&st)[4]) const {
+    return t.dim() == 4 && t.scalar_type() == dtype && t.device() == like.device() &&
+           t.numel() != 0 && t.size(3) == D && t.size(0) <= INT32_MAX && t.size(1) <= INT32_MAX &&
+           kernel_strides(t, st) && aligned(t);
+  }
+  bool counts(const Tensor &t) const {
+    return t.dim() == 1 && t.size(0) == B && t.scalar_type() == at::kInt &&
+           t.device() == like.device() && (B == 1 || t.stride(0) == 1);
+  }
+  bool table(const Tensor &t) const {
+    return t.dim() == 2 && t.size(0) == B && t.size(1) == cache->width &&
+           t.scalar_type() == at::kInt && t.device() == like.device() && t.stride(0) >= 0 &&
+           (t.stride(1) == 1 || t.size(1) == 1);
+  }
+};
+
+const int32_t *ints(const OptTensor &t) { return t ? t->data_ptr<int32_t>() : nullptr; }
+
+// (done, q_out or None)
+std::tuple<bool, OptTensor> paged_append(int64_t cache, const Tensor &like, bool half, int64_t D,
+                                         const Tensor &table, const Tensor &k, const Tensor &v,
+                                         const OptTensor &q, const Tensor &start,
+                                         const OptTensor &counts, const OptTensor &steps,
+                                         double factor, int64_t dim, int64_t flags) {
+  PagedCall c{reinterpret_cast<const fa_paged_cache *>(cache), like,
+              half ? at::kHalf : at::kBFloat16, D};
+  int64_t k_st[4], v_st[4], q_st[4] = {}, qo_st[4] = {};
+  const std::tuple<bool, OptTensor> no{false, OptTensor()};
+  if (!like.is_cuda() || !c.rows(k, k_st) || !c.rows(v, v_st) || k.sizes() != v.sizes() ||
+      k.size(2) != c.cache->heads)
+    return no;
+  const int64_t S = k.size(1);
+  c.B = k.size(0);
+  if (!c.table(table) || !c.counts(start) || (counts && !c.counts(*counts)) ||
+      (steps && (steps->device() != like.device() || dim > D)))
+    return no;
+  if (q && (!c.rows(*q, q_st) || q->size(0) != c.B || q->size(1) != S)) return no;
+  const c10::DeviceGuard guard(like.device());
+  Tensor out;
+  if (q) {
+    out = at::empty(q->sizes(), q->options());
+    kernel_strides(out, qo_st);
+  }
+  check(fa_paged_append(c.cache, table.data_ptr<int32_t>(), table.stride(0), k.data_ptr(),
+                        v.data_ptr(), q ? q->data_ptr() : nullptr, q ? out.data_ptr() : nullptr,
+                        ints(OptTensor(start)), ints(counts),
+                        steps ? steps->data_ptr<int64_t>() : nullptr, factor, (int)dim, (int)flags,
+                        (int)c.B, (int)S, q ? (int)q->size(2) : 0, (int)D, k_st, v_st, q_st, qo_st,
+                        c.code(), stream_of(like)),
+        "fa_paged_append");
+  return {true, q ? OptTensor(out) : OptTensor()};
+}
+
+std::optional<std::tuple<Tensor, Tensor>> paged_read(int64_t cache, const Tensor &like, bool half,
+                                                     int64_t D, const Tensor &table,
+                                                     const Tensor &start, int64_t n,
+                                                     const OptTensor &counts) {
+  PagedCall c{reinterpret_cast<const fa_paged_cache *>(cache), like,
+              half ? at::kHalf : at::kBFloat16, D};
+  c.B = table.dim() == 2 ? table.size(0) : 0;
+  if (!like.is_cuda() || c.B <= 0 || n <= 0 || n > INT32_MAX || !c.table(table) ||
+      !c.counts(start) || (counts && !c.counts(*counts)))
+    return std::nullopt;
+  const c10::DeviceGuard guard(like.device());
+  const auto opt = like.options().dtype(c.dtype);
+  Tensor k = at::empty({c.B, n, c.cache->heads, D}, opt), v = at::empty(k.sizes(), opt);
+  check(fa_paged_read(c.cache, table.data_ptr<int32_t>(), table.stride(0), k.data_ptr(),
+                      v.data_ptr(), ints(OptTensor(start)), ints(counts), (int)c.B, (int)n, (int)D,
+                      c.code(), stream_of(like)),
+        "fa_paged_read");
+  return std::make_tuple(k, v);
+}
+
+std::optional<std::tuple<Tensor, OptTensor>> paged_attend(int64_t cache, const Tensor &like,
+                                                          bool half, int64_t D, const Tensor &q,
+                                                          const Tensor &table,
+                                                          const Tensor &lengths,
+                                                          const OptTensor &counts, double scale,
+                                                          bool want_lse) {
+  PagedCall c{reinterpret_cast<const fa_paged_cache *>(cache), like,
+              half ? at::kHalf : at::kBFloat16, D};
+  int64_t q_st[4];
+  if (!like.is_cuda() || !c.rows(q, q_st)) return std::nullopt;
+  const int64_t Sq = q.size(1), H = q.size(2), Hk = c.cache->heads;
+  c.B = q.size(0);
+  if (H > INT32_MAX || H % Hk != 0 || !c.table(table) || !c.counts(lengths) ||
+      (counts && !c.counts(*counts)))
+    return std::nullopt;
+  const c10::DeviceGuard guard(like.device());
+  Tensor out = at::empty(q.sizes(), q.options()), lse, ws;
+  if (want_lse) lse = at::empty({c.B, H, Sq}, q.options().dtype(at::kFloat));
+  // (its memory is the allocator's again on return, for later work of this stream)
+  const size_t nb = fa_paged_attn_workspace_bytes((int)c.B, (int)Sq, (int)H, (int)Hk, (int)D);
+  if (nb) ws = at::empty({(int64_t)nb}, q.options().dtype(at::kByte));
+  check(fa_paged_attn(q.data_ptr(), c.cache, table.data_ptr<int32_t>(), table.stride(0),
+                      lengths.data_ptr<int32_t>(), ints(counts), out.data_ptr(),
+                      want_lse ? lse.data_ptr<float>() : nullptr, nb ? ws.data_ptr() : nullptr, nb,
+                      (int)c.B, (int)Sq, (int)H, (int)D, q_st, (float)scale, c.code(),
+                      stream_of(like)),
+        "fa_paged_attn");
+  return std::make_tuple(out, want_lse ? OptTensor(lse) : OptTensor());
 }
 
 }  // namespace
@@ -490,7 +639,10 @@ PYBIND11_MODULE(_fa_torch, m) {
             "apply_rotary_positions";
   m.def("make_plan", &make_plan, "register a launch plan (ints, sm_scale) -> handle");
   m.def("rope", &rope, "QK-norm + rotary prologue, recording the C++ backward node, or None");
-  m.def("rotary", &rotary, "rotation by positions, recording the C++ backward node");
+  m.def("rotary", &rotary, "rotation by positions, recording the C++ backward node, or None");
+  m.def("paged_append", &paged_append, "append_paged -> (done, q_out or None)");
+  m.def("paged_read", &paged_read, "read_paged -> (k, v), or None");
+  m.def("paged_attend", &paged_attend, "attend_paged -> (out, lse or None), or None");
   m.def("held_on_another_stream", &held_on_another_stream,
         "a leaf's gradient accumulator was made on another stream");
   m.def("attn", &attn, "forward of a plan, recording the C++ backward node");

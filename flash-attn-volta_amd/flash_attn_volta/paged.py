@@ -28,7 +28,7 @@ import math
 import torch
 
 from . import _capi, _runtime
-from ._runtime import VP
+from .autograd import _compiling, _cpp
 from .forward import (NATIVE_HEAD_DIMS, _DTYPES, _kernel_ready, _on_device, _require, _stream_ptr,
                       kernel_strides)
 from .rotary import RotaryPositions
@@ -62,7 +62,7 @@ class PagedKVCache:
     """
 
     __slots__ = ("k_codes", "k_scales", "v_codes", "v_scales", "dtype", "num_pages", "page_size",
-                 "num_kv_heads", "head_dim", "device", "_structs")
+                 "num_kv_heads", "head_dim", "device", "_structs", "_addrs", "_half")
 
     def __init__(self, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int,
                  dtype: torch.dtype = torch.bfloat16, device="cuda"):
@@ -108,7 +108,7 @@ class PagedKVCache:
             setattr(self, name, t)
         self.dtype, self.device = dtype, codes.device
         self.num_pages, self.num_kv_heads, self.page_size, self.head_dim = N, H, P, D
-        self._structs = {}
+        self._structs, self._addrs, self._half = {}, {}, dtype == torch.float16
 
     @property
     def nbytes(self) -> int:
@@ -124,6 +124,21 @@ class PagedKVCache:
                 self.k_codes.data_ptr(), self.k_scales.data_ptr(), self.v_codes.data_ptr(),
                 self.v_scales.data_ptr(), self.num_pages, self.page_size, self.num_kv_heads, width)
         return s
+
+    def _addr(self, table) -> int:
+        """Address of _struct(width of `table`); 0 where that is no table."""
+        if not isinstance(table, torch.Tensor) or table.dim() != 2 or table.shape[1] == 0:
+            return 0
+        width = table.shape[1]
+        a = self._addrs.get(width)
+        if a is None:
+            s = self._struct(width)
+            if len(self._addrs) >= 64:
+                self._addrs.clear()
+            a, _ = self._addrs[width] = (ctypes.addressof(s), s)
+        else:
+            a = a[0]
+        return a
 
     def __repr__(self):
         return (f"PagedKVCache({self.num_pages} pages of {self.page_size} tokens, "
@@ -173,6 +188,20 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def _fast(cache, page_table, *tensors) -> int:
+    """The address that the C++ calls of _fa_torch take for this cache and table,
+    0 where a call goes the general way: the C++ module is not there, the call is
+    being traced, or the arguments are not what they should be (the general
+    way names what is wrong).  The C++ calls also leave to it whatever needs a
+    copy or is empty."""
+    if _cpp is None or type(cache) is not PagedKVCache or _compiling():
+        return 0
+    for t in tensors:
+        if not isinstance(t, torch.Tensor):
+            return 0
+    return cache._addr(page_table)
+
+
 def append_paged(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor,
                  start: torch.Tensor, counts: torch.Tensor | None = None, *,
                  q: torch.Tensor | None = None,
@@ -200,6 +229,16 @@ def append_paged(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, page_tab
     largest value.  Pages that sequences share must not be appended to by
     more than one of them at the same slot: either's values may stay.
     """
+    addr = _fast(cache, page_table, k, v, start)
+    if addr and (q is None or isinstance(q, torch.Tensor)) \
+            and (counts is None or isinstance(counts, torch.Tensor)) \
+            and (rotary is None or isinstance(rotary, RotaryPositions)):
+        done, out = _cpp.paged_append(
+            addr, cache.k_codes, cache._half, cache.head_dim, page_table, k, v, q, start, counts,
+            *((None, 1.0, 0, 0) if rotary is None else
+              (rotary.steps, rotary.attention_factor, rotary.rotary_dim, rotary._flags)))
+        if done:
+            return out
     _require(isinstance(k, torch.Tensor), "k must be a tensor")
     _cache(cache, k.device)
     _rows(k, "k", cache, cache.num_kv_heads)
@@ -247,6 +286,12 @@ def read_paged(cache: PagedKVCache, page_table: torch.Tensor, start: torch.Tenso
     each (B, length, Hk, D) contiguous in the cache's dtype, exactly what the
     attention sees; 0 behind counts[b] tokens and where the table names no page.
     For moving a sequence, a dense prefill over its prefix, or inspection."""
+    addr = _fast(cache, page_table, start)
+    if addr and isinstance(length, int) and (counts is None or isinstance(counts, torch.Tensor)):
+        out = _cpp.paged_read(addr, cache.k_codes, cache._half, cache.head_dim, page_table, start,
+                              length, counts)
+        if out is not None:
+            return out
     _require(isinstance(page_table, torch.Tensor) and page_table.dim() == 2,
              "page_table must be a (B, pages) int32 tensor")
     _cache(cache, page_table.device)
@@ -305,6 +350,14 @@ def attend_paged(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tensor,
     H, D) contiguous in q's dtype and, if asked, lse (B, H, Sq) fp32; a query
     that sees no key, and every one behind ``counts``, gets 0 and +inf.
     """
+    addr = _fast(cache, page_table, q, lengths)
+    if addr and (counts is None or isinstance(counts, torch.Tensor)):
+        out = _cpp.paged_attend(
+            addr, cache.k_codes, cache._half, cache.head_dim, q, page_table, lengths, counts,
+            cache.head_dim ** -0.5 if sm_scale is None else float(sm_scale),
+            bool(return_softmax_lse))
+        if out is not None:
+            return out if return_softmax_lse else out[0]
     _require(isinstance(q, torch.Tensor), "q must be a tensor")
     _cache(cache, q.device)
     _rows(q, "q", cache)

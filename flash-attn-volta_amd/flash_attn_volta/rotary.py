@@ -271,17 +271,20 @@ def apply_rotary_positions(q: torch.Tensor, k: torch.Tensor | None, positions: t
         (q_out, k_out): contiguous (B, S, H, D) / (B, S, Hk, D) in q's dtype
         (k_out None without k).  Gradients flow to q and k.
     """
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        _check(q, k, rotary)
-        positions = _positions(positions, q.shape[0], q.shape[1], q.device)
-        if _cpp is not None and not _compiling() and _runtime.capturing():
-            for t in (q, k):
-                _require(t is None or not _cpp.held_on_another_stream(t),
-                         "an autograd graph of q or k, made on another stream, is alive: a "
-                         "backward pass cannot be captured beside it; drop its outputs first")
-        if _cpp is not None and q.numel() and (k is None or k.numel()) \
-                and not _transforms_active() and not _compiling():
-            return _cpp.rotary(q, k, positions, rotary.steps, rotary.attention_factor,
-                               rotary.rotary_dim, rotary._flags)
-        return _RotaryFn.apply(q, k, positions, rotary, False)
-    return rotary_forward(q, k, positions, rotary)
+    if _cpp is not None and isinstance(rotary, RotaryPositions) and not _transforms_active() \
+            and not _compiling() and all(isinstance(t, torch.Tensor) for t in (q, positions)) \
+            and (k is None or isinstance(k, torch.Tensor)):
+        out = _cpp.rotary(q, k, positions, rotary.steps, rotary.attention_factor,
+                          rotary.rotary_dim, rotary._flags)
+        if out is not None:
+            return out
+    _check(q, k, rotary)
+    positions = _positions(positions, q.shape[0], q.shape[1], q.device)
+    if not (torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))):
+        return _launch(q, k, positions, rotary, False)
+    if _cpp is not None and not _compiling() and _runtime.capturing():
+        for t in (q, k):
+            _require(t is None or not _cpp.held_on_another_stream(t),
+                     "an autograd graph of q or k, made on another stream, is alive: a "
+                     "backward pass cannot be captured beside it; drop its outputs first")
+    return _RotaryFn.apply(q, k, positions, rotary, False)
