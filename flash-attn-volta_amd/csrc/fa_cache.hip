@@ -203,7 +203,12 @@ AttnPlan attn_plan(int B, int Sq, int H, int Hk, int cus) {
   p.nt = p.rows <= 16 ? 1 : (p.rows <= 32 ? 2 : 0);
   const int tile = p.nt ? 16 * p.nt : fa::kRowsTile;
   p.row_tiles = (int)((p.rows + tile - 1) / tile);
-  const int64_t want = (int64_t)(p.nt ? 8 : 3) * cus / ((int64_t)Hk * p.row_tiles);
+  // As many chunks as workgroups are resident at once: a second, short round
+  // costs more than the longer sweeps.  The few-row kernel has 4 a compute unit
+  // (2 with two column tiles), the many-row one 2.  A sequence's last chunk is
+  // shorter, one more for each of the B.
+  const int64_t resident = (int64_t)(p.nt == 1 ? 4 : 2) * cus / ((int64_t)Hk * p.row_tiles);
+  const int64_t want = resident - B > resident / 2 ? resident - B : resident / 2;
   p.target = want < 1 ? 1 : (int)want;
   p.slots = p.target > 1 ? p.target + B : B;
   return p;

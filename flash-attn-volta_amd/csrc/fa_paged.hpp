@@ -316,17 +316,28 @@ constexpr float kLowest = -3.4028234663852886e38f;
 struct Chunk {
   int b, index, count, keys;            // `count` chunks of `keys` keys in sequence b
   int first;                            // slot of the sequence's chunk 0
+  int length, held;                     // lengths[b], and what of it the table holds
 };
 
-__device__ __forceinline__ int held_keys(const PagedAttnArgs &a, int b) {
+__device__ __forceinline__ int held_keys(const PagedAttnArgs &a, int length) {
   const int64_t cap = (int64_t)a.cache.width << a.cache.page_shift;
-  return (int)max((int64_t)0, min((int64_t)a.lengths[b], cap));
+  return (int)max((int64_t)0, min((int64_t)length, cap));
 }
 
-__device__ __forceinline__ int wave_sum(int x) {
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) x += __shfl_xor(x, m, 64);
-  return x;
+// Inclusive prefix sum over the wave: within rows of 16 lanes (row_shr 1, 2, 4,
+// 8; lanes without a source add 0), then each row's last into the rows behind
+// (row_bcast 15, 31).
+template <int CTRL, int ROWS> __device__ __forceinline__ int dpp_add(int x) {
+  return x + __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xF, false);
+}
+
+__device__ __forceinline__ int wave_prefix(int x) {
+  x = dpp_add<0x111, 0xF>(x);
+  x = dpp_add<0x112, 0xF>(x);
+  x = dpp_add<0x114, 0xF>(x);
+  x = dpp_add<0x118, 0xF>(x);
+  x = dpp_add<0x142, 0xA>(x);
+  return dpp_add<0x143, 0xC>(x);
 }
 
 // Splits all sequences' keys evenly: chunks of the same whole number of units
@@ -334,42 +345,55 @@ __device__ __forceinline__ int wave_sum(int x) {
 // host knows no lengths; every wave counts them for itself (B loads) and finds
 // the sequence of its slot; one that holds nothing is a chunk too, which writes
 // its zeros.  target + B slots cover every chunk, B with a target of 1 (then no
-// sequence is split).  With
-// `by_sequence` the argument is a sequence and its chunks are returned.
+// sequence is split).  With `by_sequence` the argument is a sequence and its
+// chunks are returned.
 __device__ __forceinline__ bool find_chunk(const PagedAttnArgs &a, int want, bool by_sequence,
                                            Chunk &out) {
   const int lane = threadIdx.x & 63;
-  int total = 0;
+  auto units_of = [&](int held) { return (held + kUnit - 1) / kUnit; };
+  if (a.B == 1) {                       // one user's tokens: scalar work alone
+    out.b = out.first = 0;
+    out.length = a.lengths[0];
+    out.held = held_keys(a, out.length);
+    const int u = units_of(out.held), units = max(1, (u + a.target - 1) / a.target);
+    out.count = max(1, (u + units - 1) / units);
+    out.index = want;
+    out.keys = units * kUnit;
+    return by_sequence || want < out.count;
+  }
+  int total = 0, length = 0, held = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
     const int b = b0 + lane;
-    total += b < a.B ? (held_keys(a, b) + kUnit - 1) / kUnit : 0;
+    length = b < a.B ? a.lengths[b] : 0;
+    held = held_keys(a, length);
+    total += units_of(held);
   }
-  total = wave_sum(total);
+  total = __builtin_amdgcn_readlane(wave_prefix(total), 63);
   const int units = max(1, (total + a.target - 1) / a.target);
   int before = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
     const int b = b0 + lane;
-    const int u = b < a.B ? (held_keys(a, b) + kUnit - 1) / kUnit : 0;
-    const int n = b < a.B ? max(1, (u + units - 1) / units) : 0;
-    int upto = n;                       // inclusive prefix sum
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-      const int o = __shfl_up(upto, m, 64);
-      if (lane >= m) upto += o;
+    if (a.B > 64) {                     // (else the lanes still hold theirs)
+      length = b < a.B ? a.lengths[b] : 0;
+      held = held_keys(a, length);
     }
+    const int n = b < a.B ? max(1, (units_of(held) + units - 1) / units) : 0;
+    const int upto = wave_prefix(n);
     const int first = before + upto - n;
     const bool mine = by_sequence ? b == want : (want >= first && want < first + n);
     const uint64_t hit = __ballot(mine);
     if (hit) {
       const int src = __builtin_ctzll(hit);
-      out.b = __builtin_amdgcn_readfirstlane(b0 + src);
-      out.first = __builtin_amdgcn_readfirstlane(__shfl(first, src, 64));
-      out.count = __builtin_amdgcn_readfirstlane(__shfl(n, src, 64));
+      out.b = b0 + src;
+      out.first = __builtin_amdgcn_readlane(first, src);
+      out.count = __builtin_amdgcn_readlane(n, src);
+      out.length = __builtin_amdgcn_readlane(length, src);
+      out.held = __builtin_amdgcn_readlane(held, src);
       out.index = want - out.first;
-      out.keys = __builtin_amdgcn_readfirstlane(units) * kUnit;
+      out.keys = units * kUnit;
       return true;
     }
-    before += __shfl(upto, 63, 64);
+    before += __builtin_amdgcn_readlane(upto, 63);
   }
   return false;
 }
@@ -381,28 +405,46 @@ template <> struct KRaw<32> { uint32_t w; };
 template <int D> __device__ __forceinline__ uint32_t raw_word(const KRaw<D> &r, int i) { return r.w[i]; }
 template <> __device__ __forceinline__ uint32_t raw_word<32>(const KRaw<32> &r, int) { return r.w; }
 
-// One wave's share of a 16-key tile: codes of key m's quarter g of the columns,
-// of V group g's unit m, and their scales.
+// One wave's share of a 16-key tile: codes of key m's quarter g of the columns
+// and of V group g's unit m, each with its scales.
 template <int D> struct Tile16 {
   KRaw<D> k, v;
   uint32_t ks, vs;
   bool hole;
 };
 
+// Row of 16-key tile `key` in its page, and whether it is a hole: no key, or a page
+// that is none (page 0 is read instead, its keys masked).
+__device__ __forceinline__ int64_t tile_row(const PagedCache &c, int b, int hk, int key, int end,
+                                            bool &hole) {
+  // (the id is loaded whether it is needed or not: no branch in the sweeps; as a
+  // constant: a scalar load)
+  typedef const __attribute__((address_space(4))) int32_t *Constants;
+  const int page = reinterpret_cast<Constants>(
+      reinterpret_cast<uintptr_t>(c.table))[b * c.table_stride + min(key >> c.page_shift, c.width - 1)];
+  hole = key >= end || (unsigned)page >= (unsigned)c.n_pages;
+  return paged_row(c, hole ? 0 : page, hk, key & ((1 << c.page_shift) - 1));
+}
+
+template <int D>
+__device__ __forceinline__ void load_k(const PagedCache &c, int64_t row, int m, int g, Tile16<D> &t) {
+  t.k = *reinterpret_cast<const KRaw<D> *>(c.k_codes + row * (D / 2) + m * (D / 2) + g * (D / 8));
+  t.ks = (c.k_scales + row * (D / 32))[m * (D / 32) + g * D / 128];
+}
+
+template <int D>
+__device__ __forceinline__ void load_v(const PagedCache &c, int64_t row, int m, int g, Tile16<D> &t) {
+  t.v = *reinterpret_cast<const KRaw<D> *>(c.v_codes + row * (D / 2) + (g * 16 + m) * (D / 8));
+  t.vs = *reinterpret_cast<const uint32_t *>(c.v_scales + row * (D / 32) +
+                                             (g * (D / 32) + m * D / 512) * 4);
+}
+
 template <int D>
 __device__ __forceinline__ void load_tile(const PagedCache &c, int b, int hk, int key, int end,
                                           int m, int g, Tile16<D> &t) {
-  // (a page that is none: page 0 is read instead, its keys masked)
-  int page = key < end ? page_of(c, b, key) : -1;
-  page = __builtin_amdgcn_readfirstlane(page);
-  t.hole = page < 0;
-  const int64_t row = paged_row(c, max(page, 0), hk, key & ((1 << c.page_shift) - 1));
-  const uint8_t *kc = c.k_codes + row * (D / 2), *ksc = c.k_scales + row * (D / 32);
-  const uint8_t *vc = c.v_codes + row * (D / 2), *vsc = c.v_scales + row * (D / 32);
-  t.k = *reinterpret_cast<const KRaw<D> *>(kc + m * (D / 2) + g * (D / 8));
-  t.v = *reinterpret_cast<const KRaw<D> *>(vc + (g * 16 + m) * (D / 8));
-  t.ks = ksc[m * (D / 32) + g * D / 128];
-  t.vs = *reinterpret_cast<const uint32_t *>(vsc + (g * (D / 32) + m * D / 512) * 4);
+  const int64_t row = tile_row(c, b, hk, key, end, t.hole);
+  load_k<D>(c, row, m, g, t);
+  load_v<D>(c, row, m, g, t);
 }
 
 // Byte pair s of key r in a V unit: the codes of d = 2s, 2s + 1 of the unit.
@@ -465,9 +507,9 @@ __global__ __launch_bounds__(256) void fa_paged_few_kernel(PagedAttnArgs a) {
   Chunk ch;
   if (!find_chunk(a, slot, false, ch)) return;
   const int b = ch.b, rows = a.Sq * a.G, row0 = blockIdx.y * (16 * NT);
-  const int held = held_keys(a, b);
+  const int held = ch.held;
   const int count = a.counts ? min(max(a.counts[b], 0), a.Sq) : a.Sq;
-  const int base = a.lengths[b] - count;          // position of query 0
+  const int base = ch.length - count;             // position of query 0
 
   // Q as B operands: column n = row0 + 16 nt + m, d = (D/4) g + 8 t + 0..7
   vec8<E> qf[NT][KS];
@@ -589,14 +631,17 @@ __global__ __launch_bounds__(256) void fa_paged_few_kernel(PagedAttnArgs a) {
       s_m[w][m] = mx[nt];
       s_l[w][m] = ls;
     }
+    const int here = min(rows - row0 - 16 * nt, 16);   // rows of this column tile
+    if (m < here) {
 #pragma unroll
-    for (int t = 0; t < ND; ++t)
+      for (int t = 0; t < ND; ++t)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s_o[w][ND * (4 * g + i) + t][m] = o[nt][t][i];
+        for (int i = 0; i < 4; ++i) s_o[w][ND * (4 * g + i) + t][m] = o[nt][t][i];
+    }
     __syncthreads();
-    for (int e = tid; e < 16 * D; e += 64 * NW) {
+    for (int e = tid; e < here * D; e += 64 * NW) {
       const int d = e % D, n = e / D, row = row0 + 16 * nt + n;
-      if (row < rows) {
+      {
         float top = s_m[0][n];
 #pragma unroll
         for (int k = 1; k < NW; ++k) top = fmaxf(top, s_m[k][n]);
@@ -632,19 +677,22 @@ __global__ __launch_bounds__(256) void fa_paged_few_kernel(PagedAttnArgs a) {
 // Many query rows (prompt chunks): workgroup (slot x head, row tile of 128 rows),
 // 4 waves of 32 rows.  Bound by arithmetic, half of it not matrix products, so
 // the codes are turned into 16-bit values once a workgroup: wave w converts keys
-// 16w .. 16w + 15 of each 64-key tile into LDS, one tile ahead of the products
-// and with the next tile's codes in flight.  LDS holds both operands as their
+// 16w .. 16w + 15 of each 64-key tile into LDS.  LDS holds both operands as their
 // 16-byte fragments: K as [column chunk of 8][key], V as [4-key pairs][column][8
 // keys], so every fragment is one conflict-free 16-byte read.
-// O^T tile dt, row rr is column (D/16)(rr / 2) + 2 dt + rr % 2: the order in
-// which code bytes give them.
+// The loop is pipelined so that each stretch between branches holds matrix
+// instructions and others that do not wait for them: the scores of tile j + 1
+// beside the exponentials of tile j, then the products with V of tile j beside
+// the conversion of K of tile j + 2 and V of tile j + 1.
+// O^T tile dt, row 16 e + mm is column (D/16) mm + 2 dt + e: the order in which
+// code bytes give them.
 constexpr int kRowsTile = 128, kRowsKeys = 64;
 
 template <typename E, int D>
 __global__ __launch_bounds__(256, 2) void fa_paged_rows_kernel(PagedAttnArgs a) {
   constexpr int NS = D / 16, ND = D / 32;
   __shared__ u32x4 s_k[2][D / 8][kRowsKeys];
-  __shared__ u32x2 s_v[2][kRowsKeys / 8][ND][32][2];   // [16-key part, h][dt][rr][4 keys, +8]
+  __shared__ u32x4 s_v[2][kRowsKeys / 8][ND][32];      // [16-key part, h][dt][row]: 4 keys, +8
   __shared__ int s_hole[2][4];
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -655,9 +703,8 @@ __global__ __launch_bounds__(256, 2) void fa_paged_rows_kernel(PagedAttnArgs a) 
   if (!find_chunk(a, slot, false, ch)) return;
   const int b = ch.b, rows = a.Sq * a.G;
   const int row0 = (gridDim.y - 1 - blockIdx.y) * kRowsTile;   // the longest sweeps first
-  const int held = held_keys(a, b);
   const int count = a.counts ? min(max(a.counts[b], 0), a.Sq) : a.Sq;
-  const int base = a.lengths[b] - count;
+  const int base = ch.length - count;
 
   const int row = row0 + 32 * w + n, qi = row / a.G;
   const int h = hk * a.G + (row - qi * a.G);
@@ -677,110 +724,148 @@ __global__ __launch_bounds__(256, 2) void fa_paged_rows_kernel(PagedAttnArgs a) 
   }
   const int key0 = ch.index * ch.keys;
   const int i_first = row0 / a.G, i_last = min((row0 + kRowsTile - 1) / a.G, count - 1);
-  const int end = i_first < count ? min(min(held, key0 + ch.keys), base + i_last + 1) : 0;
+  const int end = i_first < count ? min(min(ch.held, key0 + ch.keys), base + i_last + 1) : 0;
   // this wave's rows see every key below `all` and none from `wend` on
   const int wi = (row0 + 32 * w) / a.G;
   const int all = base + wi + 1;
   const int wend = wi < count ? min(end, base + min((row0 + 32 * w + 31) / a.G, count - 1) + 1) : 0;
 
   float mx = kLowest, l = 0.0f;
-  floatx16 o[ND];
+  floatx16 o[ND], s[2];
 #pragma unroll
   for (int t = 0; t < ND; ++t) o[t] = floatx16{};
 
-  Tile16<D> raw;
-  auto load = [&](int key) { load_tile<D>(a.cache, b, hk, key + 16 * w, end, m, g, raw); };
-  auto convert = [&](int buf) {
-    const float sc = fp4_scale(raw.ks);
-#pragma unroll
-    for (int t = 0; t < D / 32; ++t)
-      s_k[buf][(D / 32) * g + t][16 * w + m] = fp4_row8<E>(raw_word<D>(raw.k, t), sc);
-    float vs[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) vs[r] = fp4_scale((raw.vs >> (8 * r)) & 0xFFu);
-    auto columns = [&](auto S) {
-      constexpr int s = decltype(S)::value;
-      uint32_t x[4];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) x[r] = v_pair<E, D, s>(raw.v, r, vs[r]);
-      u32x2 *to = &s_v[buf][2 * w + (g & 1)][s][2 * m][g >> 1];
-      to[0] = u32x2{__builtin_amdgcn_perm(x[1], x[0], 0x05040100u),
-                    __builtin_amdgcn_perm(x[3], x[2], 0x05040100u)};
-      to[2] = u32x2{__builtin_amdgcn_perm(x[1], x[0], 0x07060302u),
-                    __builtin_amdgcn_perm(x[3], x[2], 0x07060302u)};
-    };
-    columns(std::integral_constant<int, 0>{});
-    if constexpr (ND > 1) columns(std::integral_constant<int, 1>{});
-    if constexpr (ND > 2) {
-      columns(std::integral_constant<int, 2>{});
-      columns(std::integral_constant<int, 3>{});
-    }
-    if (lane == 0) s_hole[buf][w] = raw.hole;
+  Tile16<D> raw;                        // K of the tile to convert, V of the one before it
+  int64_t v_row = 0;                    // where that V is, until it is loaded
+  auto load_keys = [&](int key) {
+    const int64_t r = tile_row(a.cache, b, hk, key + 16 * w, end, raw.hole);
+    load_k<D>(a.cache, r, m, g, raw);
+    return r;
   };
-
-  if (key0 < end) {
-    load(key0);
-    convert(0);
-    if (key0 + kRowsKeys < end) load(key0 + kRowsKeys);
-  }
-  __syncthreads();
-  int buf = 0;
-  for (int key = key0; key < end; key += kRowsKeys) {
-    if (key + kRowsKeys < end) {
-      convert(buf ^ 1);
-      if (key + 2 * kRowsKeys < end) load(key + 2 * kRowsKeys);
-    }
-    if (key < wend) {
-      floatx16 s[2];
+  // pieces of a tile's conversion: K chunk t of this lane's quarter of the
+  // columns; columns 2t, 2t + 1 of this lane's V unit
+  auto convert_k = [&](int buf, auto T) {
+    constexpr int t = decltype(T)::value;
+    s_k[buf][ND * g + t][16 * w + m] = fp4_row8<E>(raw_word<D>(raw.k, t), fp4_scale(raw.ks));
+    if constexpr (t == 0) s_hole[buf][w] = raw.hole;    // (every lane the same)
+  };
+  auto convert_v = [&](int buf, auto T) {
+    constexpr int t = decltype(T)::value;
+    uint32_t x[4];
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt) {
-        s[kt] = floatx16{};
-#pragma unroll
-        for (int t = 0; t < NS; ++t)
-          s[kt] = mfma32(__builtin_bit_cast(vec8<E>, s_k[buf][2 * t + hf][32 * kt + n]), qf[t], s[kt]);
-      }
-      const bool holes = s_hole[buf][0] | s_hole[buf][1] | s_hole[buf][2] | s_hole[buf][3];
-      if (key + kRowsKeys > all || key + kRowsKeys > end || __builtin_amdgcn_readfirstlane(holes)) {
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int kk = key + 32 * kt + c_row(i, hf);
-            if (kk > last || kk >= end || s_hole[buf][2 * kt + i / 8]) s[kt][i] = kNegInf;
-          }
-      }
-      float top = s[0][0];
-#pragma unroll
-      for (int i = 1; i < 32; ++i) top = fmaxf(top, s[i >> 4][i & 15]);
-      top *= a.c;
-      // a new maximum only where the old one is left behind by 2^8
-      if (__any(top > mx + 8.0f)) {
-        const float t = fmaxf(max_xor32(top), mx);
-        const float f = fast_exp2(mx - t);
-        mx = t;
-        l *= f;
-#pragma unroll
-        for (int t2 = 0; t2 < ND; ++t2) o[t2] *= f;
-      }
+    for (int r = 0; r < 4; ++r)
+      x[r] = v_pair<E, D, t>(raw.v, r, fp4_scale((raw.vs >> (8 * r)) & 0xFFu));
+    // columns 2t (lo) and 2t + 1 (hi) of keys 4g .. 4g + 3; the halves of the wave
+    // swap, so that lanes 0-31 hold 8 keys of the first, 32-63 of the second
+    auto x0 = __builtin_amdgcn_permlane32_swap(__builtin_amdgcn_perm(x[1], x[0], 0x05040100u),
+                                               __builtin_amdgcn_perm(x[1], x[0], 0x07060302u),
+                                               false, false);
+    auto x1 = __builtin_amdgcn_permlane32_swap(__builtin_amdgcn_perm(x[3], x[2], 0x05040100u),
+                                               __builtin_amdgcn_perm(x[3], x[2], 0x07060302u),
+                                               false, false);
+    s_v[buf][2 * w + (g & 1)][t][16 * hf + m] = u32x4{x0[0], x1[0], x0[1], x1[1]};
+  };
+  auto convert = [&](int kbuf, int vbuf) {
+    static_for<ND>([&](auto T) { convert_k(kbuf, T); });
+    static_for<ND>([&](auto T) { convert_v(vbuf, T); });
+  };
+  auto k_frag = [&](int buf, int i) {   // of score instruction i: columns i / 2, keys i % 2
+    return __builtin_bit_cast(vec8<E>, s_k[buf][2 * (i >> 1) + hf][32 * (i & 1) + n]);
+  };
+  auto v_frag = [&](int buf, int i) {   // of V instruction i: keys i / ND, tile i % ND
+    return __builtin_bit_cast(vec8<E>, s_v[buf][2 * (i / ND) + hf][i % ND][n]);
+  };
+  // masks tile `key`'s scores, and moves the running maximum where they leave the
+  // old one behind by 2^8
+  auto settle = [&](int key, int buf, floatx16 (&x)[2]) {
+    const int holes = s_hole[buf][0] | s_hole[buf][1] | s_hole[buf][2] | s_hole[buf][3];
+    if (key + kRowsKeys > all || key + kRowsKeys > end || __builtin_amdgcn_readfirstlane(holes)) {
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          vec8<E> p;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float e = fast_exp2(s[kt][8 * u + i] * a.c - mx);
-            l += e;
-            p[i] = (E)e;
-          }
-#pragma unroll
-          for (int t = 0; t < ND; ++t)
-            o[t] = mfma32(*reinterpret_cast<const vec8<E> *>(&s_v[buf][4 * kt + 2 * u + hf][t][n][0]),
-                          p, o[t]);
+        for (int i = 0; i < 16; ++i) {
+          const int kk = key + 32 * kt + c_row(i, hf);
+          if (kk > last || kk >= end || s_hole[buf][2 * kt + i / 8]) x[kt][i] = kNegInf;
         }
     }
+    float top = x[0][0];
+#pragma unroll
+    for (int i = 1; i < 32; ++i) top = fmaxf(top, x[i >> 4][i & 15]);
+    top *= a.c;
+    if (__any(top > mx + 8.0f)) {
+      const float t = fmaxf(max_xor32(top), mx);
+      const float f = fast_exp2(mx - t);
+      mx = t;
+      l *= f;
+#pragma unroll
+      for (int t2 = 0; t2 < ND; ++t2) o[t2] *= f;
+    }
+  };
+
+  if (key0 < end) {
+    // K of tiles 0 and 1, V of tile 0 converted; K of tile 2 and V of tile 1 loaded
+    int64_t r = load_keys(key0);
+    load_v<D>(a.cache, r, m, g, raw);
+    convert(0, 0);
+    r = load_keys(key0 + kRowsKeys);
+    static_for<ND>([&](auto T) { convert_k(1, T); });
+    load_v<D>(a.cache, r, m, g, raw);
+    v_row = load_keys(key0 + 2 * kRowsKeys);
+  }
+  __syncthreads();
+  if (key0 < wend) {
+    s[0] = s[1] = floatx16{};
+#pragma unroll
+    for (int i = 0; i < 2 * NS; ++i) s[i & 1] = mfma32(k_frag(0, i), qf[i >> 1], s[i & 1]);
+    settle(key0, 0, s);
+  }
+  __syncthreads();                      // K of tile 0 is overwritten next
+  int buf = 0;
+  for (int key = key0; key < end; key += kRowsKeys, buf ^= 1) {
+    if (key < wend) {
+      // The order is fixed here: fragments are read kAhead instructions before
+      // the matrix instruction that takes them, and each of those is followed
+      // by its share of the other work, which runs beside it.
+      constexpr int kAhead = 4, kScore = 2 * NS, kProd = 4 * ND;
+      floatx16 next[2];
+      next[0] = next[1] = floatx16{};
+      vec8<E> p[4], kf[kScore], vf[kProd];
+      static_for<kAhead>([&](auto I) { kf[I] = k_frag(buf ^ 1, I); });
+      static_for<kScore>([&](auto I) {
+        constexpr int i = decltype(I)::value, per = 32 / kScore;
+        if constexpr (i + kAhead < kScore)
+          kf[i + kAhead] = k_frag(buf ^ 1, i + kAhead);
+        else
+          vf[i + kAhead - kScore] = v_frag(buf, i + kAhead - kScore);
+        next[i & 1] = mfma32(kf[i], qf[i >> 1], next[i & 1]);
+#pragma unroll
+        for (int j = per * i; j < per * (i + 1); ++j) {
+          const float e = fast_exp2(s[j >> 4][j & 15] * a.c - mx);
+          l += e;
+          p[j >> 3][j & 7] = (E)e;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      });
+      static_for<kProd>([&](auto I) {
+        constexpr int i = decltype(I)::value;
+        if constexpr (i + kAhead < kProd) vf[i + kAhead] = v_frag(buf, i + kAhead);
+        o[i % ND] = mfma32(vf[i], p[i / ND], o[i % ND]);
+        if constexpr (i % 2 == 1 && i < 2 * ND) convert_k(buf, std::integral_constant<int, i / 2>{});
+        if constexpr (i % 2 == 1 && i >= 2 * ND)
+          convert_v(buf ^ 1, std::integral_constant<int, i / 2 - ND>{});
+        __builtin_amdgcn_sched_barrier(0);
+      });
+      load_v<D>(a.cache, v_row, m, g, raw);
+      v_row = load_keys(key + 3 * kRowsKeys);
+      s[0] = next[0];
+      s[1] = next[1];
+      if (key + kRowsKeys < wend) settle(key + kRowsKeys, buf ^ 1, s);
+    } else {
+      convert(buf, buf ^ 1);
+      load_v<D>(a.cache, v_row, m, g, raw);
+      v_row = load_keys(key + 3 * kRowsKeys);
+    }
     __syncthreads();
-    buf ^= 1;
   }
 
   if (row >= rows) return;
@@ -790,15 +875,15 @@ __global__ __launch_bounds__(256, 2) void fa_paged_rows_kernel(PagedAttnArgs a) 
   const float f = whole ? (seen ? 1.0f / l : 0.0f) : (real ? 1.0f : 0.0f);
   const int64_t part = ((int64_t)slot * Hk + hk) * rows + row;
   E *out = reinterpret_cast<E *>(a.o) + (((int64_t)b * a.Sq + qi) * a.H + h) * D;
-  // registers 2j, 2j + 1 of every dt are 2 ND consecutive columns
+  // registers j and j + 8 of every dt are 2 ND consecutive columns
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const int d = NS * (c_row(2 * j, hf) / 2);
+    const int d = NS * c_row(j, hf);
     float x[2 * ND];
 #pragma unroll
     for (int t = 0; t < ND; ++t) {
-      x[2 * t] = seen || !whole ? o[t][2 * j] * f : 0.0f;
-      x[2 * t + 1] = seen || !whole ? o[t][2 * j + 1] * f : 0.0f;
+      x[2 * t] = seen || !whole ? o[t][j] * f : 0.0f;
+      x[2 * t + 1] = seen || !whole ? o[t][j + 8] * f : 0.0f;
     }
     if (whole) {
       E y[2 * ND];
@@ -833,14 +918,26 @@ __global__ __launch_bounds__(256) void fa_paged_merge_kernel(PagedAttnArgs a) {
   const int d4 = tid % (D / 4), sub = tid / (D / 4);
   float top = kLowest, sum = 0.0f;
   floatx4 acc = {0, 0, 0, 0};
-  for (int k = sub; k < ch.count; k += NS) {
-    const int64_t p = ((int64_t)(ch.first + k) * Hk + hk) * rows + row;
-    const float mk = a.part_ml[p * 2], lk = a.part_ml[p * 2 + 1];
-    const floatx4 x = *reinterpret_cast<const floatx4 *>(a.part_o + p * D + 4 * d4);
-    const float t = fmaxf(top, mk), f0 = fast_exp2(top - t), f1 = fast_exp2(mk - t);
-    top = t;
-    sum = sum * f0 + lk * f1;
-    acc = acc * f0 + x * f1;
+  for (int k0 = sub; k0 < ch.count; k0 += 4 * NS) {      // 4 chunks' loads in flight
+    float mk[4], lk[4];
+    floatx4 x[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int k = min(k0 + j * NS, ch.count - 1);
+      const int64_t p = ((int64_t)(ch.first + k) * Hk + hk) * rows + row;
+      const floatx2 ml = *reinterpret_cast<const floatx2 *>(a.part_ml + p * 2);
+      mk[j] = ml[0];
+      lk[j] = ml[1];
+      x[j] = *reinterpret_cast<const floatx4 *>(a.part_o + p * D + 4 * d4);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (k0 + j * NS >= ch.count) break;
+      const float t = fmaxf(top, mk[j]), f0 = fast_exp2(top - t), f1 = fast_exp2(mk[j] - t);
+      top = t;
+      sum = sum * f0 + lk[j] * f1;
+      acc = acc * f0 + x[j] * f1;
+    }
   }
   __shared__ floatx4 s_acc[NS][D / 4];
   __shared__ float s_top[NS], s_sum[NS];
