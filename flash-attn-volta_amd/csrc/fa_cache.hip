@@ -100,8 +100,8 @@ int log2_up(int n) {
 
 template <typename E>
 int launch_rotary(fa::RotaryArgs a, int D, hipStream_t st) {
-  a.units = fa::rotary_units(a.rot.r2, a.rot.interleaved, D);
-  a.unit_shift = log2_up(a.units);
+  a.D = D;
+  a.unit_shift = log2_up(fa::rotary_units(D));
   // One token to a workgroup, its heads over several, until the workgroups
   // fill the GPU; then 4, whose angles are one each for the 256 lanes at
   // R = 128.
@@ -345,8 +345,7 @@ int fa_paged_append(const fa_paged_cache *cache, const int32_t *table, int64_t t
   const int64_t kv = tok * cache->heads * (D / 8);
   int64_t qu = 0;
   if (q != nullptr) {
-    a.units = fa::rotary_units(a.rot.r2, a.rot.interleaved, D);
-    a.unit_shift = log2_up(a.units);
+    a.unit_shift = log2_up(fa::rotary_units(D));
     qu = tok * H << a.unit_shift;
   }
   int64_t each = 4 * fa::kAppendThreads;

@@ -69,7 +69,7 @@ struct AppendArgs {
   RotaryTable rot;                       // steps NULL: no rotation
   int S, H;
   int parts;                             // of gridDim.y, those that store keys and values
-  int units, unit_shift;                 // of a row of q (rotary_units)
+  int unit_shift;                        // log2 of the lanes for a row of q
   float top;                             // largest finite value that is kept
   int max_byte;                          // largest scale byte
 };
@@ -132,61 +132,84 @@ __global__ __launch_bounds__(kAppendThreads) void fa_paged_append_kernel(AppendA
     // queries (rows behind the count too: they are results, not cache)
     if (nt <= 0) return;
     CosSin<float> *cs = reinterpret_cast<CosSin<float> *>(smem);
-    for (int i = tid; i < nt * r2; i += kAppendThreads) {
-      const int t = i / r2, j = i - t * r2;
-      cs[t * slots + pair_slot(j, r2)] =
-          rotary_cos_sin<float>(start + i0 + t, a.rot.steps[j], (float)a.rot.factor);
-    }
-    if (r2) __syncthreads();
     const int u = tid & ((1 << a.unit_shift) - 1), lanes = kAppendThreads >> a.unit_shift;
-    if (u >= a.units) return;
-    const int step = lanes * (gridDim.y - a.parts), dt = step / a.H, dh = step - dt * a.H;
-    int t = (blockIdx.y - a.parts) * lanes + (tid >> a.unit_shift), h = t % a.H;
-    t /= a.H;
-    for (; t < nt; t += dt, h += dh) {
-      if (h >= a.H) {
-        h -= a.H;
-        if (++t >= nt) break;
-      }
-      rotate_unit<E>(a.q + b * a.qs[0] + (int64_t)(i0 + t) * a.qs[1] + h * a.qs[2],
-                     a.q_out + b * a.qos[0] + (int64_t)(i0 + t) * a.qos[1] + h * a.qos[2], u,
-                     cs + t * slots, r2, a.rot.interleaved != 0);
-    }
+    const int step = lanes * (gridDim.y - a.parts), dt = step / a.H;
+    const int first = (blockIdx.y - a.parts) * lanes + (tid >> a.unit_shift), t0 = first / a.H;
+    const f16 *q = a.q + b * a.qs[0] + (int64_t)i0 * a.qs[1];
+    f16 *out = a.q_out + b * a.qos[0] + (int64_t)i0 * a.qos[1];
+    rotate_rows<E>(
+        RotaryUnit(u, r2, a.rot.interleaved, D), u < rotary_units(D), t0, first - t0 * a.H, dt,
+        step - dt * a.H, nt, a.H, cs, slots, r2, a.rot.interleaved != 0,
+        [&](int t, int h) { return q + t * a.qs[1] + h * a.qs[2]; },
+        [&](int t, int h) { return out + t * a.qos[1] + h * a.qos[2]; },
+        [&] {
+          for (int i = tid; i < nt * r2; i += kAppendThreads) {
+            const int t = i / r2, j = i - t * r2;
+            cs[t * slots + pair_slot(j, r2)] =
+                rotary_cos_sin<float>(start + i0 + t, a.rot.steps[j], (float)a.rot.factor);
+          }
+          if (r2) __syncthreads();
+        });
     return;
   }
   if (a.counts) nt = min(nt, a.counts[b] - i0);
   if (nt <= 0) return;
   CosSin<double> *cs = reinterpret_cast<CosSin<double> *>(smem);
+  // 8 aligned positions are slots of one page
+  const int64_t pos0 = start + i0;
+  const int page = page_of(a.cache, b, pos0);
+  const int slot0 = (int)(pos0 & ((1 << a.cache.page_shift) - 1));
+  // Lane: chunk c of rows first, first + (dt, dh), ..: token t of head h.
+  // Whole blocks of 32 columns stay together, in groups of 4 lanes.
+  constexpr int kRows = kAppendThreads / NCH;
+  const int Hk = a.cache.Hk, c = tid % NCH, step = kRows * a.parts;
+  const int dh = step / nt, dt = step - dh * nt;
+  const int first = blockIdx.y * kRows + tid / NCH;
+  int h = first / nt, t = first - h * nt;
+  const f16 *k = a.k + b * a.ks[0] + (int64_t)i0 * a.ks[1], *v = a.v + b * a.vs[0] + (int64_t)i0 * a.vs[1];
+  const int other = partner_chunk(c, r2, a.rot.interleaved != 0);
+  u32x4 kx, kz, vx;                      // the next row's
+  auto fetch = [&] {
+    if (h < Hk) {
+      const f16 *kr = k + t * a.ks[1] + h * a.ks[2];
+      kx = load_raw8(kr + 8 * c);
+      kz = load_raw8(kr + other);
+      vx = load_raw8(v + t * a.vs[1] + h * a.vs[2] + 8 * c);
+    }
+  };
+  fetch();
   for (int i = tid; i < nt * r2; i += kAppendThreads) {
-    const int t = i / r2, j = i - t * r2;
-    cs[t * slots + pair_slot(j, r2)] =
-        rotary_cos_sin<double>(start + i0 + t, a.rot.steps[j], a.rot.factor);
+    const int j = i / r2, p = i - j * r2;
+    cs[j * slots + pair_slot(p, r2)] =
+        rotary_cos_sin<double>(pos0 + j, a.rot.steps[p], a.rot.factor);
   }
   if (r2) __syncthreads();
-  const int Hk = a.cache.Hk;
-  // whole blocks of 32 columns stay together: nt * Hk * NCH is a multiple of 4
-  for (int i = blockIdx.y * kAppendThreads + tid; i < nt * Hk * NCH; i += a.parts * kAppendThreads) {
-    const int c = i % NCH, th = i / NCH, h = th / nt, t = th - h * nt;
-    const int64_t pos = start + i0 + t;
-    const int page = page_of(a.cache, b, pos);
-    const int slot = (int)(pos & ((1 << a.cache.page_shift) - 1));
-    const f16 *kr = a.k + b * a.ks[0] + (int64_t)(i0 + t) * a.ks[1] + h * a.ks[2];
-    const f16 *vr = a.v + b * a.vs[0] + (int64_t)(i0 + t) * a.vs[1] + h * a.vs[2];
+  while (h < Hk) {
+    const int ht = h, tt = t;
     float vy[8], ky[8];
-    load8<E, float>(vr + 8 * c, vy);
+    unpack8<E, float>(vx, vy);
+    const u32x4 x = kx, z = kz;
+    h += dh;
+    t += dt;
+    if (t >= nt) {
+      t -= nt;
+      ++h;
+    }
+    fetch();
     if (r2) {
       double y[8];
-      rotate8<E, double>(kr, c, cs + t * slots, r2, a.rot.interleaved != 0, y);
+      rotate8<E, double>(x, z, k + tt * a.ks[1] + ht * a.ks[2], c, cs + tt * slots, r2,
+                         a.rot.interleaved != 0, y);
 #pragma unroll
       for (int j = 0; j < 8; ++j) ky[j] = odd_float(y[j]);
     } else {
-      load8<E, float>(kr + 8 * c, ky);
+      unpack8<E, float>(x, ky);
     }
     unsigned kb, vb;
     const uint32_t kw = quantise8(ky, a.top, a.max_byte, kb);
     const uint32_t vw = quantise8(vy, a.top, a.max_byte, vb);
     if (page < 0) continue;
-    const int64_t row = paged_row(a.cache, page, h, slot);
+    const int64_t row = paged_row(a.cache, page, ht, slot0 + tt);
     *reinterpret_cast<uint32_t *>(a.cache.k_codes + row * (D / 2) + 4 * c) = kw;
     // group row / 4, token r = row % 4: unit m of a group is 4 tokens x D/32 bytes
     const int64_t group = row >> 2;

@@ -68,11 +68,13 @@ __device__ __forceinline__ CosSin<F> rotary_cos_sin(int64_t p, int64_t step, F f
 }
 
 template <typename E, typename F>
-__device__ __forceinline__ void load8(const f16 *p, F *x) {
-  const vec8<E> v = *reinterpret_cast<const vec8<E> *>(p);
+__device__ __forceinline__ void unpack8(u32x4 raw, F *x) {
+  const vec8<E> v = __builtin_bit_cast(vec8<E>, raw);
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = (F)(float)v[i];
 }
+
+__device__ __forceinline__ u32x4 load_raw8(const f16 *p) { return *reinterpret_cast<const u32x4 *>(p); }
 
 // Place of pair j in a row's table of cosines and sines in LDS: lanes that own
 // consecutive chunks of 8 columns read consecutive entries.
@@ -80,17 +82,25 @@ __device__ __forceinline__ int pair_slot(int j, int r2) { return (j & 7) * ((r2 
 // Entries of a row's table.
 __host__ __device__ __forceinline__ int pair_slots(int r2) { return 8 * ((r2 + 7) >> 3); }
 
-// Columns 8c .. 8c+7 of a row, rotated by the row's table cs.  The partner
-// columns of a half-layout chunk are a load of their own (they come from the L1
-// line that another lane of the wave loads as its own chunk): a lane then owns 8
-// consecutive columns whatever R is, and groups of 4 lanes own the 32-column
-// blocks that the 4-bit cache shares a scale over.  Chunks whose partners
-// are not 8 aligned columns (R % 16) load them one by one; the branch is uniform.
+// Offset of the chunk that holds the partners of columns 8c .. 8c+7, where they
+// are one aligned chunk (half layout, R % 16 = 0, c in the rotated columns); 8c
+// itself elsewhere.
+__device__ __forceinline__ int partner_chunk(int c, int r2, bool interleaved) {
+  const int d = 8 * c;
+  if (interleaved || (r2 & 7) != 0 || d >= 2 * r2) return d;
+  return d < r2 ? d + r2 : d - r2;
+}
+
+// Columns 8c .. 8c+7 of a row (`raw`), rotated by the row's table cs; `other` is
+// partner_chunk's.  A lane then owns 8 consecutive columns whatever R is, and
+// groups of 4 lanes the 32-column blocks that the 4-bit cache shares a scale
+// over.  Partners that are no aligned chunk are loaded one by one; the branches
+// but d < R are uniform.
 template <typename E, typename F>
-__device__ __forceinline__ void rotate8(const f16 *row, int c, const CosSin<F> *cs, int r2,
-                                        bool interleaved, F *y) {
+__device__ __forceinline__ void rotate8(u32x4 raw, u32x4 other, const f16 *row, int c,
+                                        const CosSin<F> *cs, int r2, bool interleaved, F *y) {
   F x[8];
-  load8<E, F>(row + 8 * c, x);
+  unpack8<E, F>(raw, x);
   if (interleaved) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -109,7 +119,7 @@ __device__ __forceinline__ void rotate8(const f16 *row, int c, const CosSin<F> *
     if (d < 2 * r2) {
       const bool low = d < r2;
       F z[8];
-      load8<E, F>(row + (low ? d + r2 : d - r2), z);
+      unpack8<E, F>(other, z);
       const CosSin<F> *t = cs + ((low ? d : d - r2) >> 3);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -136,46 +146,100 @@ __device__ __forceinline__ void rotate8(const f16 *row, int c, const CosSin<F> *
 }
 
 template <typename E>
-__device__ __forceinline__ void store8(f16 *p, const float *y) {
+__device__ __forceinline__ u32x4 pack8(const float *y) {
   vec8<E> v;
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = (E)y[i];
-  *reinterpret_cast<vec8<E> *>(p) = v;
+  return __builtin_bit_cast(u32x4, v);
 }
 
-// Units of a row, one lane's work each: in the half layout with R % 16 = 0 two
-// chunks of 8 columns that are each other's partners (each is loaded, and its
-// cosines read, once) or one behind R; else one chunk.
-__host__ __device__ __forceinline__ int rotary_units(int r2, bool interleaved, int D) {
-  return !interleaved && (r2 & 7) == 0 ? D / 8 - r2 / 8 : D / 8;
-}
+__device__ __forceinline__ void store_raw8(f16 *p, u32x4 v) { *reinterpret_cast<u32x4 *>(p) = v; }
 
-template <typename E>
-__device__ __forceinline__ void rotate_unit(const f16 *row, f16 *out, int u,
-                                            const CosSin<float> *cs, int r2, bool interleaved) {
-  const int pairs = r2 >> 3;
-  if (!interleaved && (r2 & 7) == 0) {
-    if (u < pairs) {
-      float x[8], z[8], y[8];
-      load8<E, float>(row + 8 * u, x);
-      load8<E, float>(row + 8 * u + r2, z);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const CosSin<float> v = cs[u + i * pairs];
-        y[i] = x[i] * v.c - z[i] * v.s;
-        z[i] = z[i] * v.c + x[i] * v.s;
-      }
-      store8<E>(out + 8 * u, y);
-      store8<E>(out + 8 * u + r2, z);
-    } else {
-      const int d = 8 * (u + pairs);
-      *reinterpret_cast<u32x4 *>(out + d) = *reinterpret_cast<const u32x4 *>(row + d);
-    }
-  } else {
-    float y[8];
-    rotate8<E, float>(row, u, cs, r2, interleaved, y);
-    store8<E>(out + 8 * u, y);
+// Units of a row, one lane's work each: two chunks of 8 columns (one in rows of
+// an odd number of chunks).  In the half layout with R % 16 = 0 the two are each
+// other's partners, so that each is loaded, and its cosines read, once.
+__host__ __device__ __forceinline__ int rotary_units(int D) { return D % 16 ? D / 8 : D / 16; }
+
+struct RotaryUnit {
+  int c0, c1;        // chunks; c1 = -1: none
+  bool pair;
+  __device__ __forceinline__ RotaryUnit(int u, int r2, bool interleaved, int D) {
+    const int pairs = r2 >> 3;
+    const bool half = !interleaved && (r2 & 7) == 0;
+    pair = half && D % 16 == 0 && u < pairs;
+    c0 = D % 16 ? u : (pair ? u : 2 * u);
+    c1 = D % 16 ? -1 : (pair ? u + pairs : 2 * u + 1);
   }
+};
+
+// Rotates unit `u` of rows first, first + (dt, dh), .. of nt tokens x heads:
+// in(t, h) and out(t, h) give a row's place, `ready` waits for the tables cs + t *
+// slots.  2 rows' loads are in flight at a time, the first before the wait: a row
+// is a few hundred bytes, and one at a time the sweep would wait for each.
+template <typename E, typename In, typename Out, typename Ready>
+__device__ __forceinline__ void rotate_rows(const RotaryUnit u, bool active, int t, int h, int dt,
+                                            int dh, int nt, int heads, const CosSin<float> *cs,
+                                            int slots, int r2, bool interleaved, In &&in,
+                                            Out &&out, Ready &&ready) {
+  constexpr int N = 2;
+  bool waited = false;
+  if (!active) t = nt;
+  do {
+    u32x4 x[N], z[N];
+    int ts[N], hs[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if (h >= heads) {
+        h -= heads;
+        ++t;
+      }
+      ts[j] = t;
+      hs[j] = h;
+      if (t < nt) {
+        const f16 *row = in(t, h);
+        x[j] = load_raw8(row + 8 * u.c0);
+        if (u.c1 >= 0) z[j] = load_raw8(row + 8 * u.c1);
+      }
+      t += dt;
+      h += dh;
+    }
+    if (!waited) ready();
+    waited = true;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if (ts[j] >= nt) break;
+      const CosSin<float> *c = cs + ts[j] * slots;
+      f16 *to = out(ts[j], hs[j]);
+      if (u.pair) {
+        float a[8], b[8], y[8];
+        unpack8<E, float>(x[j], a);
+        unpack8<E, float>(z[j], b);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const CosSin<float> v = c[u.c0 + i * (r2 >> 3)];
+          y[i] = a[i] * v.c - b[i] * v.s;
+          b[i] = b[i] * v.c + a[i] * v.s;
+        }
+        store_raw8(to + 8 * u.c0, pack8<E>(y));
+        store_raw8(to + 8 * u.c1, pack8<E>(b));
+      } else {
+        // chunks behind R are copied as they are
+        const f16 *row = in(ts[j], hs[j]);
+#pragma unroll 1
+        for (int k = 0; k < (u.c1 >= 0 ? 2 : 1); ++k) {
+          const int chunk = k ? u.c1 : u.c0;
+          u32x4 raw = k ? z[j] : x[j];
+          if (8 * chunk < 2 * r2) {
+            float y[8];
+            rotate8<E, float>(raw, load_raw8(row + partner_chunk(chunk, r2, interleaved)), row,
+                              chunk, c, r2, interleaved, y);
+            raw = pack8<E>(y);
+          }
+          store_raw8(to + 8 * chunk, raw);
+        }
+      }
+    }
+  } while (t < nt);
 }
 
 struct RotaryArgs {
@@ -188,7 +252,7 @@ struct RotaryArgs {
   const void *positions;
   int64_t pb, ps;       // strides of positions
   int pos64;            // int64 positions
-  int S, units, unit_shift;   // units of a row, and log2 of the lanes for them
+  int S, D, unit_shift;   // log2 of the lanes for a row's units
   int64_t tokens;       // B * S
 };
 
@@ -208,7 +272,7 @@ template <typename E, int TOK>
 __global__ __launch_bounds__(kRotaryThreads) void fa_rotary_kernel(RotaryArgs a) {
   extern __shared__ char smem[];
   CosSin<float> *cs = reinterpret_cast<CosSin<float> *>(smem);   // [TOK][pair_slots]
-  __shared__ int64_t s_x[TOK][2], s_y[TOK][2];                   // a token's row offsets
+  __shared__ int64_t s_x[TOK][2], s_y[TOK][2], s_p[TOK];         // a token's offsets
   const int r2 = a.rot.r2, slots = pair_slots(r2), tid = threadIdx.x;
   const int64_t n0 = (int64_t)blockIdx.x * TOK;
   const int nt = (int)min((int64_t)TOK, a.tokens - n0);
@@ -219,32 +283,35 @@ __global__ __launch_bounds__(kRotaryThreads) void fa_rotary_kernel(RotaryArgs a)
       s_x[tid][i] = b * a.xs[i][0] + s * a.xs[i][1];
       s_y[tid][i] = b * a.ys[i][0] + s * a.ys[i][1];
     }
-  }
-  for (int i = tid; i < nt * r2; i += kRotaryThreads) {
-    const int t = i / r2, j = i - t * r2;
-    const uint32_t n = (uint32_t)(n0 + t), b = n / (uint32_t)a.S, s = n - b * (uint32_t)a.S;
-    const int64_t p = rotary_position(a.positions, a.pos64, b * a.pb + s * a.ps);
-    CosSin<float> v = rotary_cos_sin<float>(p, a.rot.steps[j], (float)a.rot.factor);
-    if (a.rot.inverse) v.s = -v.s;
-    cs[t * slots + pair_slot(j, r2)] = v;
+    s_p[tid] = b * a.pb + s * a.ps;
   }
   __syncthreads();
   const int u = tid & ((1 << a.unit_shift) - 1), lanes = kRotaryThreads >> a.unit_shift;
-  if (u >= a.units) return;
   const int heads = a.heads[0] + a.heads[1], step = lanes * gridDim.y;
-  const int dt = step / heads, dh = step - dt * heads;
-  int t = (blockIdx.y * lanes + (tid >> a.unit_shift)), hh = t % heads;
-  t /= heads;
-  for (; t < nt; t += dt, hh += dh) {
-    if (hh >= heads) {
-      hh -= heads;
-      if (++t >= nt) break;
-    }
-    const int side = hh >= a.heads[0], h = side ? hh - a.heads[0] : hh;
-    rotate_unit<E>(a.x[side] + s_x[t][side] + h * a.xs[side][2],
-                   a.y[side] + s_y[t][side] + h * a.ys[side][2], u, cs + t * slots, r2,
-                   a.rot.interleaved != 0);
-  }
+  const int dt = step / heads, first = blockIdx.y * lanes + (tid >> a.unit_shift);
+  const int t0 = first / heads;
+  auto side = [&](int h) { return h >= a.heads[0] ? 1 : 0; };
+  rotate_rows<E>(
+      RotaryUnit(u, r2, a.rot.interleaved, a.D), u < rotary_units(a.D), t0, first - t0 * heads, dt,
+      step - dt * heads, nt, heads, cs, slots, r2, a.rot.interleaved != 0,
+      [&](int t, int h) {
+        const int i = side(h);
+        return a.x[i] + s_x[t][i] + (h - (i ? a.heads[0] : 0)) * a.xs[i][2];
+      },
+      [&](int t, int h) {
+        const int i = side(h);
+        return a.y[i] + s_y[t][i] + (h - (i ? a.heads[0] : 0)) * a.ys[i][2];
+      },
+      [&] {
+        for (int i = tid; i < nt * r2; i += kRotaryThreads) {
+          const int t = i / r2, j = i - t * r2;
+          const int64_t p = rotary_position(a.positions, a.pos64, s_p[t]);
+          CosSin<float> v = rotary_cos_sin<float>(p, a.rot.steps[j], (float)a.rot.factor);
+          if (a.rot.inverse) v.s = -v.s;
+          cs[t * slots + pair_slot(j, r2)] = v;
+        }
+        __syncthreads();
+      });
 }
 
 }  // namespace fa
