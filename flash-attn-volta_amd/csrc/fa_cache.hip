@@ -104,7 +104,9 @@ int launch_rotary(fa::RotaryArgs a, int D, hipStream_t st) {
   a.unit_shift = log2_up(fa::rotary_units(D));
   // One token to a workgroup, its heads over several, until the workgroups
   // fill the GPU; then 4, whose angles are one each for the 256 lanes at
-  // R = 128.
+  // R = 128, or 8 of at most 128 units, which would leave lanes without work
+  // (8 x 1001 tokens, 24 heads of 64: 14.5 / 12.7 us with 4 / 8; 4096, 40 of 128:
+  // 17.5 / 21.4).
   const int cus = stream_cus(st);
   const int64_t rows = (int64_t)a.heads[0] + a.heads[1], lanes = fa::kRotaryThreads >> a.unit_shift;
   const size_t lds = fa::pair_slots(a.rot.r2) * sizeof(fa::CosSin<float>);
@@ -114,6 +116,9 @@ int launch_rotary(fa::RotaryArgs a, int D, hipStream_t st) {
     y = y > most ? most : (y < 1 ? 1 : y);
     fa::fa_rotary_kernel<E, 1>
         <<<dim3((unsigned)a.tokens, (unsigned)y), fa::kRotaryThreads, lds, st>>>(a);
+  } else if (rows << a.unit_shift <= 128) {
+    fa::fa_rotary_kernel<E, 8>
+        <<<dim3((unsigned)((a.tokens + 7) / 8)), fa::kRotaryThreads, 8 * lds, st>>>(a);
   } else {
     fa::fa_rotary_kernel<E, 4>
         <<<dim3((unsigned)((a.tokens + 3) / 4)), fa::kRotaryThreads, 4 * lds, st>>>(a);
@@ -233,8 +238,17 @@ int launch_attn(const fa::PagedAttnArgs &a, const AttnPlan &p, hipStream_t st) {
     fa::fa_paged_rows_kernel<E, D><<<grid, 256, 0, st>>>(a);
   if (int rc = launch_status()) return rc;
   if (p.target == 1) return FA_OK;
-  fa::fa_paged_merge_kernel<E, D>
-      <<<dim3((unsigned)p.rows, (unsigned)a.cache.Hk, (unsigned)a.B), 256, 0, st>>>(a);
+  // Rows joined by a workgroup: one, its chunks over 1024 / D groups of lanes, or
+  // as many as there are groups where that fills the GPU.
+  constexpr int kGroups = 1024 / D;
+  const int64_t all = p.rows * a.cache.Hk * a.B;
+  if (all >= (int64_t)4 * kGroups * stream_cus(st))
+    fa::fa_paged_merge_kernel<E, D, 1>
+        <<<dim3((unsigned)((p.rows + kGroups - 1) / kGroups), (unsigned)a.cache.Hk, (unsigned)a.B),
+           256, 0, st>>>(a);
+  else
+    fa::fa_paged_merge_kernel<E, D, kGroups>
+        <<<dim3((unsigned)p.rows, (unsigned)a.cache.Hk, (unsigned)a.B), 256, 0, st>>>(a);
   return launch_status();
 }
 
@@ -349,7 +363,7 @@ int fa_paged_append(const fa_paged_cache *cache, const int32_t *table, int64_t t
     qu = tok * H << a.unit_shift;
   }
   int64_t each = 4 * fa::kAppendThreads;
-  while (each > fa::kAppendThreads && (kv + qu) / each * tiles * B < 8 * stream_cus(st)) each /= 2;
+  while (each > fa::kAppendThreads && (kv + qu) / each * tiles * B < 2 * stream_cus(st)) each /= 2;
   auto parts = [&](int64_t n) { return n > 64 * each ? 64 : (n + each - 1) / each; };
   a.parts = (int)parts(kv);
   const dim3 grid((unsigned)tiles, (unsigned)(a.parts + parts(qu)), (unsigned)B);

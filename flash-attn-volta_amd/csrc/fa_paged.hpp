@@ -926,19 +926,21 @@ __global__ __launch_bounds__(256, 2) void fa_paged_rows_kernel(PagedAttnArgs a) 
   }
 }
 
-// Joins the chunks of row blockIdx.x of head blockIdx.y of sequence blockIdx.z
-// (rows whose sequence is one chunk were written by its workgroup).
-template <typename E, int D>
+// Joins the chunks of each row of head blockIdx.y of sequence blockIdx.z (rows
+// whose sequence is one chunk were written by its workgroup): D / 4 lanes take 4
+// columns each of every NS-th chunk of a row, NS such groups a row.  Bound by
+// latency (NS > 1: few rows of many chunks) or by reading the chunks' rows.
+template <typename E, int D, int NS>
 __global__ __launch_bounds__(256) void fa_paged_merge_kernel(PagedAttnArgs a) {
-  const int row = blockIdx.x, hk = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
+  constexpr int kLanes = D / 4, kRows = 256 / (kLanes * NS);
+  const int hk = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
   const int rows = a.Sq * a.G, Hk = a.cache.Hk;
   Chunk ch;
   find_chunk(a, b, true, ch);
-  const int i = row / a.G, h = hk * a.G + (row - i * a.G);
-  E *out = reinterpret_cast<E *>(a.o) + (((int64_t)b * a.Sq + i) * a.H + h) * D;
   if (ch.count == 1) return;
-  constexpr int NS = 256 / (D / 4);               // chunks at a time, D / 4 lanes each
-  const int d4 = tid % (D / 4), sub = tid / (D / 4);
+  const int d4 = tid % kLanes, group = tid / kLanes, sub = group % NS;
+  const int row = blockIdx.x * kRows + group / NS;
+  if (row >= rows) return;              // (NS > 1: one row, never)
   float top = kLowest, sum = 0.0f;
   floatx4 acc = {0, 0, 0, 0};
   for (int k0 = sub; k0 < ch.count; k0 += 4 * NS) {      // 4 chunks' loads in flight
@@ -962,32 +964,34 @@ __global__ __launch_bounds__(256) void fa_paged_merge_kernel(PagedAttnArgs a) {
       acc = acc * f0 + x[j] * f1;
     }
   }
-  __shared__ floatx4 s_acc[NS][D / 4];
-  __shared__ float s_top[NS], s_sum[NS];
-  s_acc[sub][d4] = acc;
-  if (d4 == 0) {
-    s_top[sub] = top;
-    s_sum[sub] = sum;
+  if constexpr (NS > 1) {
+    __shared__ floatx4 s_acc[NS][kLanes];
+    __shared__ float s_top[NS], s_sum[NS];
+    s_acc[sub][d4] = acc;
+    if (d4 == 0) {
+      s_top[sub] = top;
+      s_sum[sub] = sum;
+    }
+    __syncthreads();
+    if (sub != 0) return;
+    top = s_top[0];
+    for (int k = 1; k < NS; ++k) top = fmaxf(top, s_top[k]);
+    sum = 0.0f;
+    acc = floatx4{0, 0, 0, 0};
+    for (int k = 0; k < NS; ++k) {
+      const float f = fast_exp2(s_top[k] - top);
+      sum += s_sum[k] * f;
+      acc += s_acc[k][d4] * f;
+    }
   }
-  __syncthreads();
-  if (tid >= D / 4) return;
-  top = s_top[0];
-#pragma unroll
-  for (int k = 1; k < NS; ++k) top = fmaxf(top, s_top[k]);
-  sum = 0.0f;
-  acc = floatx4{0, 0, 0, 0};
-#pragma unroll
-  for (int k = 0; k < NS; ++k) {
-    const float f = fast_exp2(s_top[k] - top);
-    sum += s_sum[k] * f;
-    acc += s_acc[k][tid] * f;
-  }
+  const int i = row / a.G, h = hk * a.G + (row - i * a.G);
+  E *out = reinterpret_cast<E *>(a.o) + (((int64_t)b * a.Sq + i) * a.H + h) * D;
   const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
   vec4<E> v;
 #pragma unroll
   for (int j = 0; j < 4; ++j) v[j] = (E)(acc[j] * inv);
-  *reinterpret_cast<vec4<E> *>(out + 4 * tid) = v;
-  if (a.lse && tid == 0)
+  *reinterpret_cast<vec4<E> *>(out + 4 * d4) = v;
+  if (a.lse && d4 == 0)
     a.lse[((int64_t)b * a.H + h) * a.Sq + i] =
         sum == 0.0f ? kPosInf : (top + fast_log2(sum)) * kLn2;
 }
