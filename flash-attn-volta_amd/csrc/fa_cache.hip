@@ -57,6 +57,8 @@ void copy3(int64_t *to, const int64_t *st) {
   for (int i = 0; i < 3; ++i) to[i] = st[i];
 }
 
+constexpr int64_t kMaxThreads = 0xFFFFF000;   // of a grid dimension
+
 int launch_status() { return hipGetLastError() == hipSuccess ? FA_OK : FA_ERR_LAUNCH; }
 
 // Compute units of the device `stream` belongs to (the current device for
@@ -202,7 +204,7 @@ struct AttnPlan {
   }
 };
 
-AttnPlan attn_plan(int B, int Sq, int H, int Hk, int cus) {
+AttnPlan attn_plan(int B, int Sq, int H, int Hk, int cus, int64_t capacity) {
   AttnPlan p;
   p.rows = (int64_t)Sq * (H / Hk);
   p.nt = p.rows <= 16 ? 1 : (p.rows <= 32 ? 2 : 0);
@@ -214,7 +216,7 @@ AttnPlan attn_plan(int B, int Sq, int H, int Hk, int cus) {
   // shorter, one more for each of the B.
   const int64_t resident = (int64_t)(p.nt == 1 ? 4 : 2) * cus / ((int64_t)Hk * p.row_tiles);
   const int64_t want = resident - B > resident / 2 ? resident - B : resident / 2;
-  p.target = want < 1 ? 1 : (int)want;
+  p.target = want < 1 || capacity <= fa::kUnit ? 1 : (int)want;   // (a unit is never split)
   p.slots = p.target > 1 ? p.target + B : B;
   return p;
 }
@@ -283,7 +285,8 @@ int fa_rotary(const void *q, const void *k, void *q_out, void *k_out, const int6
     if (int rc = check_rows(k_out, k_out_strides, B, S, Hk, D, true)) return rc;
   }
   const int64_t tokens = (int64_t)B * S;
-  if (tokens > INT32_MAX || ((int64_t)H + Hk) * (D / 8) > (1 << 24)) return FA_ERR_TOO_LARGE;
+  // a grid has under 2^32 threads: 64 a token; rows are counted in 32 bits
+  if (tokens > kMaxThreads / 64 || ((int64_t)H + Hk) * (D / 8) > (1 << 24)) return FA_ERR_TOO_LARGE;
   fa::RotaryArgs a{};
   a.x[0] = static_cast<const f16 *>(q);
   a.y[0] = static_cast<f16 *>(q_out);
@@ -329,7 +332,7 @@ int fa_paged_append(const fa_paged_cache *cache, const int32_t *table, int64_t t
     if (int rc = check_rows(q, q_strides, B, S, H, D, false)) return rc;
     if (int rc = check_rows(q_out, q_out_strides, B, S, H, D, true)) return rc;
   }
-  if ((int64_t)(q ? H : 0) > (1 << 20) || S > (1 << 30)) return FA_ERR_TOO_LARGE;
+  if ((int64_t)(q ? H : 0) > (1 << 20) || S > (1 << 26)) return FA_ERR_TOO_LARGE;
   fa::AppendArgs a{};
   a.cache = device_cache(cache, table, table_stride);
   a.k = static_cast<const f16 *>(k);
@@ -380,7 +383,7 @@ int fa_paged_read(const fa_paged_cache *cache, const int32_t *table, int64_t tab
   if (!aligned(k, 16) || !aligned(v, 16) || !aligned(start, 4) || !aligned(counts, 4))
     return FA_ERR_ALIGNMENT;
   const double work = (double)B * n * cache->heads * (D / 8);
-  if (work / 256 >= 4.0e9 / 2) return FA_ERR_TOO_LARGE;
+  if (work > (double)kMaxThreads) return FA_ERR_TOO_LARGE;
   const fa::ReadArgs a{device_cache(cache, table, table_stride), static_cast<f16 *>(k),
                        static_cast<f16 *>(v), start, counts, n,
                        (int64_t)B * n * cache->heads * (D / 8)};
@@ -390,7 +393,7 @@ int fa_paged_read(const fa_paged_cache *cache, const int32_t *table, int64_t tab
 
 size_t fa_paged_attn_workspace_bytes(int B, int Sq, int H, int Hk, int D) {
   if (check_attn_sizes(B, Sq, H, Hk, D, FA_DTYPE_F16) != FA_OK) return 0;
-  return attn_plan(B, Sq, H, Hk, stream_cus(nullptr)).bytes(Hk, D);
+  return attn_plan(B, Sq, H, Hk, stream_cus(nullptr), INT64_MAX).bytes(Hk, D);
 }
 
 int fa_paged_attn(const void *q, const fa_paged_cache *cache, const int32_t *table,
@@ -406,11 +409,15 @@ int fa_paged_attn(const void *q, const fa_paged_cache *cache, const int32_t *tab
   if (!isfinite(sm_scale)) return FA_ERR_SCALE;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const int Hk = cache->heads;
-  const AttnPlan p = attn_plan(B, Sq, H, Hk, stream_cus(st));
-  if (p.bytes(Hk, D) > 0) {
-    if (workspace == nullptr || workspace_bytes < p.bytes(Hk, D)) return FA_ERR_WORKSPACE;
+  // (the size does not depend on the cache: a small one may leave it unused)
+  const int cus = stream_cus(st);
+  const AttnPlan most = attn_plan(B, Sq, H, Hk, cus, INT64_MAX);
+  if ((int64_t)most.slots * Hk > kMaxThreads / 256) return FA_ERR_TOO_LARGE;
+  if (most.bytes(Hk, D) > 0) {
+    if (workspace == nullptr || workspace_bytes < most.bytes(Hk, D)) return FA_ERR_WORKSPACE;
     if (!aligned(workspace, 16)) return FA_ERR_ALIGNMENT;
   }
+  const AttnPlan p = attn_plan(B, Sq, H, Hk, cus, (int64_t)cache->width * cache->page_size);
   fa::PagedAttnArgs a{};
   a.cache = device_cache(cache, table, table_stride);
   a.q = static_cast<const f16 *>(q);

@@ -61,8 +61,8 @@ class PagedKVCache:
     append_paged and must not be put there.
     """
 
-    __slots__ = ("k_codes", "k_scales", "v_codes", "v_scales", "dtype", "num_pages", "page_size",
-                 "num_kv_heads", "head_dim", "device", "_structs", "_addrs", "_half")
+    __slots__ = ("_tensors", "dtype", "num_pages", "page_size", "num_kv_heads", "head_dim", "device",
+                 "_structs", "_addrs", "_half", "_like")
 
     def __init__(self, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int,
                  dtype: torch.dtype = torch.bfloat16, device="cuda"):
@@ -105,14 +105,20 @@ class PagedKVCache:
             _require(t.device == codes.device, "the cache's tensors must be on one device")
             _require(t.is_contiguous() and t.data_ptr() % 16 == 0,
                      lambda: f"{name} must be contiguous and 16-byte aligned")
-            setattr(self, name, t)
+        # (kept as they are: the calls' structs hold their addresses)
+        self._tensors, self._like = dict(tensors), codes
         self.dtype, self.device = dtype, codes.device
         self.num_pages, self.num_kv_heads, self.page_size, self.head_dim = N, H, P, D
         self._structs, self._addrs, self._half = {}, {}, dtype == torch.float16
 
+    k_codes = property(lambda self: self._tensors["k_codes"])
+    k_scales = property(lambda self: self._tensors["k_scales"])
+    v_codes = property(lambda self: self._tensors["v_codes"])
+    v_scales = property(lambda self: self._tensors["v_scales"])
+
     @property
     def nbytes(self) -> int:
-        return sum(getattr(self, n).numel() for n in _shapes(1, 16, 1, 32))
+        return sum(t.numel() for t in self._tensors.values())
 
     def _struct(self, width: int):
         """fa_paged_cache for a table of `width` pages a sequence."""
@@ -234,7 +240,7 @@ def append_paged(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, page_tab
             and (counts is None or isinstance(counts, torch.Tensor)) \
             and (rotary is None or isinstance(rotary, RotaryPositions)):
         done, out = _cpp.paged_append(
-            addr, cache.k_codes, cache._half, cache.head_dim, page_table, k, v, q, start, counts,
+            addr, cache._like, cache._half, cache.head_dim, page_table, k, v, q, start, counts,
             *((None, 1.0, 0, 0) if rotary is None else
               (rotary.steps, rotary.attention_factor, rotary.rotary_dim, rotary._flags)))
         if done:
@@ -288,7 +294,7 @@ def read_paged(cache: PagedKVCache, page_table: torch.Tensor, start: torch.Tenso
     For moving a sequence, a dense prefill over its prefix, or inspection."""
     addr = _fast(cache, page_table, start)
     if addr and isinstance(length, int) and (counts is None or isinstance(counts, torch.Tensor)):
-        out = _cpp.paged_read(addr, cache.k_codes, cache._half, cache.head_dim, page_table, start,
+        out = _cpp.paged_read(addr, cache._like, cache._half, cache.head_dim, page_table, start,
                               length, counts)
         if out is not None:
             return out
@@ -353,7 +359,7 @@ def attend_paged(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tensor,
     addr = _fast(cache, page_table, q, lengths)
     if addr and (counts is None or isinstance(counts, torch.Tensor)):
         out = _cpp.paged_attend(
-            addr, cache.k_codes, cache._half, cache.head_dim, q, page_table, lengths, counts,
+            addr, cache._like, cache._half, cache.head_dim, q, page_table, lengths, counts,
             cache.head_dim ** -0.5 if sm_scale is None else float(sm_scale),
             bool(return_softmax_lse))
         if out is not None:

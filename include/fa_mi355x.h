@@ -480,7 +480,7 @@ int fa_rope_qk_bwd(const void *dq_out, const void *dk_out, const void *q, const 
  * q, q_out (B, S, H, D); k, k_out (B, S, Hk, D), or Hk = 0 and none.  D a
  * multiple of 8 up to 256, R even, 2 <= R <= D (else FA_ERR_HEAD_DIM).
  * FA_ROTARY_INVERSE rotates back: the gradients of q and k from those of
- * q_out and k_out.
+ * q_out and k_out.  At most 67 million tokens a call (FA_ERR_TOO_LARGE).
  *
  * No counterpart in the reference, which leaves rotary embeddings to
  * transformers' tables (flash_attn_volta/patch_hf.py:177, :291-303, :462).
@@ -553,15 +553,17 @@ int fa_paged_read(const fa_paged_cache *cache, const int32_t *table, int64_t tab
 size_t fa_paged_attn_workspace_bytes(int B, int Sq, int H, int Hk, int D);
 
 /*
- * Attention of the newest queries over the cache: sequence b holds
- * lengths[b] tokens (at most width * P are read), the last counts[b] of them (Sq with counts NULL; clamped to
- * 0 .. Sq) are those of the queries, and query i sees the positions up to
- * lengths[b] - counts[b] + i.  A query that sees none, and every query behind
- * counts[b], gets o = 0 and lse = +inf.  Scores are fp32; keys and values enter
- * the products as the exact 16-bit values of their codes (fp16: rounded below
- * 2^-24).  q (B, Sq, H, D), o (B, Sq, H, D) contiguous, lse (B, H, Sq) fp32 or
- * NULL; query head h reads head h / (H / heads).  The lengths are read on the
- * device, which shares all sequences' keys out evenly whatever they are.
+ * Attention of the newest queries over the cache.  Sequence b holds lengths[b]
+ * tokens (at most width * P are read), of which the last counts[b] (Sq with
+ * counts NULL; clamped to 0 .. Sq) are those of the queries: query i sees the
+ * positions up to lengths[b] - counts[b] + i.  A query that sees none, and
+ * every query behind counts[b], gets o = 0 and lse = +inf.  Scores are fp32; keys
+ * and values enter the products as the exact 16-bit values of their codes (fp16:
+ * rounded below 2^-24).  The lengths are read on the device, which shares all
+ * sequences' keys out evenly whatever they are.
+ * q (B, Sq, H, D); o (B, Sq, H, D) contiguous; lse (B, H, Sq) fp32 or NULL; query
+ * head h reads head h / (H / heads).  At most 2^20 rows a head of the cache (Sq
+ * H / heads) and 2^30 positions a sequence (width * P), else FA_ERR_TOO_LARGE.
  * workspace: fa_paged_attn_workspace_bytes, 16-byte aligned (NULL where 0).
  *
  * No counterpart in the reference, whose patch falls back to eager attention
