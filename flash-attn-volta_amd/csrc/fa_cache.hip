@@ -212,8 +212,9 @@ AttnPlan attn_plan(int B, int Sq, int H, int Hk, int cus, int64_t capacity) {
   p.row_tiles = (int)((p.rows + tile - 1) / tile);
   // As many chunks as workgroups are resident at once: a second, short round
   // costs more than the longer sweeps.  The few-row kernel has 4 a compute unit
-  // (2 with two column tiles), the many-row one 2.  A sequence's last chunk is
-  // shorter, one more for each of the B.
+  // (2 with two column tiles: 16 x 4 queries of 14 / 2 heads of 64 on up to 5000
+  // tokens 8.9 us, 11.4 with 4), the many-row one 2.  A sequence's last
+  // chunk is shorter, one more for each of the B.
   const int64_t resident = (int64_t)(p.nt == 1 ? 4 : 2) * cus / ((int64_t)Hk * p.row_tiles);
   const int64_t want = resident - B > resident / 2 ? resident - B : resident / 2;
   p.target = want < 1 || capacity <= fa::kUnit ? 1 : (int)want;   // (a unit is never split)

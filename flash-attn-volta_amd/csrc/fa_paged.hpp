@@ -642,58 +642,59 @@ __global__ __launch_bounds__(256) void fa_paged_few_kernel(PagedAttnArgs a) {
   }
 
   // Join the waves.  O^T tile t, register i: column (query) m, d = (D/16)(4g + i) + t.
-  __shared__ float s_o[NW][D][17];                // 17: columns of a row in different banks
-  __shared__ float s_m[NW][16], s_l[NW][16];
-  const int64_t part = ((int64_t)slot * Hk + hk) * rows;
-  const bool whole = ch.count == 1;
+  __shared__ float s_o[NW][NT][D][17];            // 17: columns of a row in different banks
+  __shared__ float s_m[NW][16 * NT], s_l[NW][16 * NT];
+  const int here = min(rows - row0, 16 * NT);     // rows of this tile
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     float ls = l[nt] + __shfl_xor(l[nt], 16, 64);
     ls += xor32(ls);
-    if (g == 0) {
-      s_m[w][m] = mx[nt];
-      s_l[w][m] = ls;
-    }
-    const int here = min(rows - row0 - 16 * nt, 16);   // rows of this column tile
-    if (m < here) {
+    if (16 * nt + m < here) {
+      if (g == 0) {
+        s_m[w][16 * nt + m] = mx[nt];
+        s_l[w][16 * nt + m] = ls;
+      }
 #pragma unroll
       for (int t = 0; t < ND; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s_o[w][ND * (4 * g + i) + t][m] = o[nt][t][i];
+        for (int i = 0; i < 4; ++i) s_o[w][nt][ND * (4 * g + i) + t][m] = o[nt][t][i];
     }
-    __syncthreads();
-    for (int e = tid; e < here * D; e += 64 * NW) {
-      const int d = e % D, n = e / D, row = row0 + 16 * nt + n;
-      {
-        float top = s_m[0][n];
+  }
+  __syncthreads();
+  // a row to every 256 / 2^k threads, 2^k >= rows: its factors once a thread
+  const int lanes = 256 >> (here > 1 ? 32 - __builtin_clz(here - 1) : 0);
+  const int n = tid / lanes, row = row0 + n;
+  if (n >= here) return;
+  const int i = row / a.G, h = hk * a.G + (row - i * a.G);
+  float top = s_m[0][n], sum = 0.0f, f[NW];
 #pragma unroll
-        for (int k = 1; k < NW; ++k) top = fmaxf(top, s_m[k][n]);
-        const int i = row / a.G, h = hk * a.G + (row - i * a.G);
-        float sum = 0.0f, acc = 0.0f;
-        if (i < count) {
+  for (int k = 1; k < NW; ++k) top = fmaxf(top, s_m[k][n]);
 #pragma unroll
-          for (int k = 0; k < NW; ++k) {
-            const float f = fast_exp2(s_m[k][n] - top);
-            sum += s_l[k][n] * f;
-            acc += s_o[k][d][n] * f;
-          }
-        }
-        if (whole) {
-          reinterpret_cast<E *>(a.o)[(((int64_t)b * a.Sq + i) * a.H + h) * D + d] =
-              (E)(sum > 0.0f ? acc / sum : (sum == 0.0f ? 0.0f : sum));
-          if (a.lse && d == 0)
-            a.lse[((int64_t)b * a.H + h) * a.Sq + i] =
-                sum == 0.0f ? kPosInf : (top + fast_log2(sum)) * kLn2;
-        } else {
-          a.part_o[(part + row) * D + d] = acc;
-          if (d == 0) {
-            a.part_ml[(part + row) * 2] = top;
-            a.part_ml[(part + row) * 2 + 1] = sum;
-          }
-        }
-      }
-    }
-    __syncthreads();
+  for (int k = 0; k < NW; ++k) {
+    f[k] = fast_exp2(s_m[k][n] - top);
+    sum += s_l[k][n] * f[k];
+  }
+  const bool real = i < count, whole = ch.count == 1;
+  const float inv = !real || sum == 0.0f ? 0.0f : (whole ? 1.0f / sum : 1.0f);   // (NaN: kept)
+  const int64_t part = ((int64_t)slot * Hk + hk) * rows + row;
+  const int64_t out = (((int64_t)b * a.Sq + i) * a.H + h) * D;
+  for (int d = tid % lanes; d < D; d += lanes) {
+    float acc = 0.0f;
+#pragma unroll
+    for (int k = 0; k < NW; ++k) acc += s_o[k][n >> 4][d][n & 15] * f[k];
+    acc = inv == 0.0f ? 0.0f : acc * inv;
+    if (whole)
+      reinterpret_cast<E *>(a.o)[out + d] = (E)acc;
+    else
+      a.part_o[part * D + d] = acc;
+  }
+  if (tid % lanes != 0) return;
+  if (!whole) {
+    a.part_ml[part * 2] = top;
+    a.part_ml[part * 2 + 1] = real ? sum : 0.0f;
+  } else if (a.lse) {
+    a.lse[((int64_t)b * a.H + h) * a.Sq + i] =
+        !real || sum == 0.0f ? kPosInf : (top + fast_log2(sum)) * kLn2;
   }
 }
 
