@@ -7,6 +7,7 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "fa_mi355x.h"
@@ -207,18 +208,22 @@ struct AttnPlan {
 AttnPlan attn_plan(int B, int Sq, int H, int Hk, int cus, int64_t capacity) {
   AttnPlan p;
   p.rows = (int64_t)Sq * (H / Hk);
-  p.nt = p.rows <= 16 ? 1 : (p.rows <= 32 ? 2 : 0);
+  // The many-row kernel pays from 65 rows on, from 257 where a call has at most
+  // 8192 in all and is bound by latency (us with the join, few rows / many: 64 rows
+  // of 32 x 8 heads on 2000 tokens 41 / 55; 128 of 64 heads on 4000 42 / 43; 192 of 64
+  // 66 / 52; 256 of 128 on 2000 73 / 59; 128, 256 of 8 heads on 8000 23 / 33, 29 / 35;
+  // 128 of 32 on 4000 29 / 35).
+  const bool few = p.rows <= 64 || (p.rows <= 256 && p.rows * Hk * B <= 8192);
+  p.nt = p.rows <= 16 ? 1 : (few ? 2 : 0);
   const int tile = p.nt ? 16 * p.nt : fa::kRowsTile;
   p.row_tiles = (int)((p.rows + tile - 1) / tile);
   // As many chunks as workgroups are resident at once: a second, short round
   // costs more than the longer sweeps.  The few-row kernel has 4 a compute unit
   // (2 with two column tiles: 16 x 4 queries of 14 / 2 heads of 64 on up to 5000
-  // tokens 8.9 us, 11.4 with 4), the many-row one 2.  A sequence's last
-  // chunk is shorter, one more for each of the B.
+  // tokens 8.9 us, 11.4 with 4), the many-row one 2.
   const int64_t resident = (int64_t)(p.nt == 1 ? 4 : 2) * cus / ((int64_t)Hk * p.row_tiles);
-  const int64_t want = resident - B > resident / 2 ? resident - B : resident / 2;
-  p.target = want < 1 || capacity <= fa::kUnit ? 1 : (int)want;   // (a unit is never split)
-  p.slots = p.target > 1 ? p.target + B : B;
+  p.target = resident < 1 || capacity <= fa::kUnit ? 1 : (int)resident;   // (a unit is never split)
+  p.slots = p.target > 1 ? std::max(p.target, (p.target + 1) / 2 + B) : B;   // fa::find_chunk
   return p;
 }
 
@@ -241,17 +246,17 @@ int launch_attn(const fa::PagedAttnArgs &a, const AttnPlan &p, hipStream_t st) {
     fa::fa_paged_rows_kernel<E, D><<<grid, 256, 0, st>>>(a);
   if (int rc = launch_status()) return rc;
   if (p.target == 1) return FA_OK;
-  // Rows joined by a workgroup: one, its chunks over 1024 / D groups of lanes, or
-  // as many as there are groups where that fills the GPU.
+  // Groups of D / 4 lanes that share a row's chunks: 8, or one where rows alone
+  // fill the GPU (256 queries of 32 heads of 128, 8 chunks: 9.4 / 6.4 us).
   constexpr int kGroups = 1024 / D;
-  const int64_t all = p.rows * a.cache.Hk * a.B;
-  if (all >= (int64_t)4 * kGroups * stream_cus(st))
-    fa::fa_paged_merge_kernel<E, D, 1>
-        <<<dim3((unsigned)((p.rows + kGroups - 1) / kGroups), (unsigned)a.cache.Hk, (unsigned)a.B),
-           256, 0, st>>>(a);
+  auto blocks = [&](int ns) {
+    const int64_t each = kGroups / ns;
+    return dim3((unsigned)((p.rows + each - 1) / each), (unsigned)a.cache.Hk, (unsigned)a.B);
+  };
+  if (p.rows * a.cache.Hk * a.B >= (int64_t)4 * kGroups * stream_cus(st))
+    fa::fa_paged_merge_kernel<E, D, 1><<<blocks(1), 256, 0, st>>>(a);
   else
-    fa::fa_paged_merge_kernel<E, D, kGroups>
-        <<<dim3((unsigned)p.rows, (unsigned)a.cache.Hk, (unsigned)a.B), 256, 0, st>>>(a);
+    fa::fa_paged_merge_kernel<E, D, 8><<<blocks(8), 256, 0, st>>>(a);
   return launch_status();
 }
 

@@ -364,59 +364,89 @@ __device__ __forceinline__ int wave_prefix(int x) {
 }
 
 // Splits all sequences' keys evenly: chunks of the same whole number of units
-// (the last of a sequence shorter), about `target` of them, whatever the lengths.  The
-// host knows no lengths; every wave counts them for itself (B loads) and finds
-// the sequence of its slot; one that holds nothing is a chunk too, which writes
-// its zeros.  target + B slots cover every chunk, B with a target of 1 (then no
-// sequence is split).  With `by_sequence` the argument is a sequence and its
-// chunks are returned.
+// (the last of a sequence shorter), `target` of them at most where that can be,
+// whatever the lengths.  The host knows no lengths; every wave counts them for
+// itself (B loads) and finds the sequence of its slot; one that holds nothing is
+// a chunk too, which writes its zeros.  max(target, (target + 1) / 2 + B) slots
+// cover every chunk, B with a target of 1 (then no sequence is split).  With
+// `by_sequence` the argument is a sequence and its chunks are returned.
 __device__ __forceinline__ bool find_chunk(const PagedAttnArgs &a, int want, bool by_sequence,
                                            Chunk &out) {
   const int lane = threadIdx.x & 63;
   auto units_of = [&](int held) { return (held + kUnit - 1) / kUnit; };
+  // ceil(u / units), 1 at least, u and units up to 2^23: an fp32 quotient, off by
+  // one at most
+  auto parts = [&](int u, int units) {
+    const int x = u + units - 1;
+    int q = (int)((float)x * __builtin_amdgcn_rcpf((float)units));
+    q -= q * units > x ? 1 : 0;
+    q += (q + 1) * units <= x ? 1 : 0;
+    return max(1, q);
+  };
   if (a.B == 1) {                       // one user's tokens: scalar work alone
     out.b = out.first = 0;
     out.length = a.lengths[0];
     out.held = held_keys(a, out.length);
-    const int u = units_of(out.held), units = max(1, (u + a.target - 1) / a.target);
-    out.count = max(1, (u + units - 1) / units);
+    const int u = units_of(out.held), units = parts(u, a.target);
+    out.count = parts(u, units);
     out.index = want;
     out.keys = units * kUnit;
     return by_sequence || want < out.count;
   }
-  int total = 0, length = 0, held = 0;
-  for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const int b = b0 + lane;
+  // Short last chunks can go over the target: then as many fewer whole ones as there
+  // are sequences, half the target at least.
+  auto fewer = [&](int total) {
+    return max(1, (total - 1) / max(a.target - a.B, (a.target + 1) / 2) + 1);
+  };
+  int length = 0, held = 0;
+  auto load = [&](int b) {              // units of sequence b, this lane's
     length = b < a.B ? a.lengths[b] : 0;
     held = held_keys(a, length);
-    total += units_of(held);
+    return units_of(held);
+  };
+  auto find = [&](int first, int n, int b0, int units) {
+    const bool mine = by_sequence ? b0 + lane == want : (want >= first && want < first + n);
+    const uint64_t hit = __ballot(mine);
+    if (!hit) return false;
+    const int src = __builtin_ctzll(hit);
+    out.b = b0 + src;
+    out.first = __builtin_amdgcn_readlane(first, src);
+    out.count = __builtin_amdgcn_readlane(n, src);
+    out.length = __builtin_amdgcn_readlane(length, src);
+    out.held = __builtin_amdgcn_readlane(held, src);
+    out.index = want - out.first;
+    out.keys = units * kUnit;
+    return true;
+  };
+  auto last = [](int x) { return __builtin_amdgcn_readlane(x, 63); };
+  if (a.B <= 64) {
+    const int u = load(lane), total = last(wave_prefix(u));
+    int units = max(1, (total + a.target - 1) / a.target);
+    int n = lane < a.B ? parts(u, units) : 0, upto = wave_prefix(n);
+    if (last(upto) > a.target) {
+      units = fewer(total);
+      n = lane < a.B ? parts(u, units) : 0;
+      upto = wave_prefix(n);
+    }
+    return find(upto - n, n, 0, units);
   }
-  total = __builtin_amdgcn_readlane(wave_prefix(total), 63);
-  const int units = max(1, (total + a.target - 1) / a.target);
+  auto sum = [&](auto &&f) {            // over all sequences
+    int x = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 64) {
+      const int u = load(b0 + lane);
+      x += b0 + lane < a.B ? f(u) : 0;
+    }
+    return last(wave_prefix(x));
+  };
+  const int total = sum([](int u) { return u; });
+  int units = max(1, (total + a.target - 1) / a.target);
+  if (sum([&](int u) { return parts(u, units); }) > a.target) units = fewer(total);
   int before = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const int b = b0 + lane;
-    if (a.B > 64) {                     // (else the lanes still hold theirs)
-      length = b < a.B ? a.lengths[b] : 0;
-      held = held_keys(a, length);
-    }
-    const int n = b < a.B ? max(1, (units_of(held) + units - 1) / units) : 0;
+    const int u = load(b0 + lane), n = b0 + lane < a.B ? parts(u, units) : 0;
     const int upto = wave_prefix(n);
-    const int first = before + upto - n;
-    const bool mine = by_sequence ? b == want : (want >= first && want < first + n);
-    const uint64_t hit = __ballot(mine);
-    if (hit) {
-      const int src = __builtin_ctzll(hit);
-      out.b = b0 + src;
-      out.first = __builtin_amdgcn_readlane(first, src);
-      out.count = __builtin_amdgcn_readlane(n, src);
-      out.length = __builtin_amdgcn_readlane(length, src);
-      out.held = __builtin_amdgcn_readlane(held, src);
-      out.index = want - out.first;
-      out.keys = units * kUnit;
-      return true;
-    }
-    before += __builtin_amdgcn_readlane(upto, 63);
+    if (find(before + upto - n, n, b0, units)) return true;
+    before += last(upto);
   }
   return false;
 }
@@ -940,11 +970,12 @@ __global__ __launch_bounds__(256) void fa_paged_merge_kernel(PagedAttnArgs a) {
   find_chunk(a, b, true, ch);
   if (ch.count == 1) return;
   const int d4 = tid % kLanes, group = tid / kLanes, sub = group % NS;
-  const int row = blockIdx.x * kRows + group / NS;
-  if (row >= rows) return;              // (NS > 1: one row, never)
+  const int mine = group / NS, row = blockIdx.x * kRows + mine;
+  const bool real = row < rows;
+  const int chunks = real ? ch.count : 0;
   float top = kLowest, sum = 0.0f;
   floatx4 acc = {0, 0, 0, 0};
-  for (int k0 = sub; k0 < ch.count; k0 += 4 * NS) {      // 4 chunks' loads in flight
+  for (int k0 = sub; k0 < chunks; k0 += 4 * NS) {        // 4 chunks' loads in flight
     float mk[4], lk[4];
     floatx4 x[4];
 #pragma unroll
@@ -966,25 +997,28 @@ __global__ __launch_bounds__(256) void fa_paged_merge_kernel(PagedAttnArgs a) {
     }
   }
   if constexpr (NS > 1) {
-    __shared__ floatx4 s_acc[NS][kLanes];
-    __shared__ float s_top[NS], s_sum[NS];
-    s_acc[sub][d4] = acc;
+    __shared__ floatx4 s_acc[kRows][NS][kLanes];
+    __shared__ float s_top[kRows][NS], s_sum[kRows][NS];
+    s_acc[mine][sub][d4] = acc;
     if (d4 == 0) {
-      s_top[sub] = top;
-      s_sum[sub] = sum;
+      s_top[mine][sub] = top;
+      s_sum[mine][sub] = sum;
     }
     __syncthreads();
     if (sub != 0) return;
-    top = s_top[0];
-    for (int k = 1; k < NS; ++k) top = fmaxf(top, s_top[k]);
+    top = s_top[mine][0];
+#pragma unroll
+    for (int k = 1; k < NS; ++k) top = fmaxf(top, s_top[mine][k]);
     sum = 0.0f;
     acc = floatx4{0, 0, 0, 0};
+#pragma unroll
     for (int k = 0; k < NS; ++k) {
-      const float f = fast_exp2(s_top[k] - top);
-      sum += s_sum[k] * f;
-      acc += s_acc[k][d4] * f;
+      const float f = fast_exp2(s_top[mine][k] - top);
+      sum += s_sum[mine][k] * f;
+      acc += s_acc[mine][k][d4] * f;
     }
   }
+  if (!real) return;
   const int i = row / a.G, h = hk * a.G + (row - i * a.G);
   E *out = reinterpret_cast<E *>(a.o) + (((int64_t)b * a.Sq + i) * a.H + h) * D;
   const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);

@@ -269,6 +269,79 @@ def test_attend_padded_batch_holes_strides(dtype, Sq, H, Hk, D):
         _check_attend(out, lse, q, model, table, lengths, counts, scale)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("Sq,H,Hk,D", [(150, 8, 4, 32), (70, 8, 2, 64), (41, 14, 2, 128)])
+def test_attend_many_rows_padded(dtype, Sq, H, Hk, D):
+    """As above with more rows than the few-row kernel takes: whole prompt chunks of
+    a padded batch, holes, empty rows, all in one chunk (a small table) and
+    split (a large one)."""
+    from flash_attn_volta import attend_paged
+    lengths, counts = [Sq + 300, 47, 3, 0, 130], [Sq, 1, 0, Sq, Sq // 2]
+    lengths[4] = 30                                        # fewer tokens than queries
+    cache, table, model = _filled(5, lengths, Hk, D, 16, dtype, 3, width=30)
+    table[0, 2], table[4, 0], table[1, 0] = -1, 2 ** 30, -2 ** 31
+    q = _rand((5, Sq, H, D), dtype, 8)
+    for n, cnt in ((lengths, counts), (lengths, None)):
+        out, lse = attend_paged(q.cuda(), cache, _i32(table), _i32(n),
+                                None if cnt is None else _i32(cnt), return_softmax_lse=True)
+        _check_attend(out, lse, q, model, table, n, cnt)
+    one = attend_paged(q[:1].cuda(), cache, _i32(table[:1]), _i32(lengths[:1]))
+    _check_attend(one, None, q[:1], model, table[:1], lengths[:1])
+
+
+def test_attend_long_prompt_split_and_whole():
+    """A prompt against itself, 128-row tiles from one query on to all; many heads
+    (one chunk a sequence) and one (split)."""
+    from flash_attn_volta import attend_paged
+    for B, Sq, H, Hk, D, dtype in ((1, 700, 2, 1, 64, F16), (3, 260, 48, 24, 32, BF16),
+                                   (1, 333, 8, 8, 128, BF16)):
+        print(f"[case] prompt {B} {Sq} {H} {Hk} {D} {dtype}", flush=True)
+        lengths = [Sq] * B
+        cache, table, model = _filled(B, lengths, Hk, D, 64, dtype, 2)
+        q = _rand((B, Sq, H, D), dtype, 6)
+        out, lse = attend_paged(q.cuda(), cache, _i32(table), _i32(lengths), return_softmax_lse=True)
+        _check_attend(out, lse, q, model, table, lengths)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_scores_that_grow_many_rows(dtype):
+    from flash_attn_volta import PagedKVCache, append_paged, attend_paged
+    L, D, Sq = 900, 128, 300
+    cache, table = PagedKVCache(60, 16, 1, D, dtype), _table(1, 57, 60, 0)
+    k = _rand((1, L, 1, D), dtype, 0).float()
+    k[..., 0] = torch.linspace(-30, 30, L)[None, :, None]
+    v = _rand((1, L, 1, D), dtype, 1)
+    q = _rand((1, Sq, 1, D), dtype, 2).float()
+    q[:, ::2, 0, 0], q[:, 1::2, 0, 0] = 12.0, -12.0
+    k, q = k.to(dtype), q.to(dtype)
+    model = orc.PagedModel(60, 16, 1, D, dtype == F16)
+    model.store(_f64(k), _f64(v), table, [0])
+    append_paged(cache, k.cuda(), v.cuda(), _i32(table), _i32([0]))
+    out, lse = attend_paged(q.cuda(), cache, _i32(table), _i32([L]), return_softmax_lse=True)
+    _check_attend(out, lse, q, model, table, [L])
+
+
+def test_a_token_that_is_not_seen_does_not_matter():
+    """Later tokens of extreme values, infinities and NaN do not reach earlier
+    queries of the same tile: the cache holds finite values, unseen ones weigh 0."""
+    from flash_attn_volta import PagedKVCache, append_paged, attend_paged
+    for dtype, Sq, H in ((F16, 8, 2), (BF16, 8, 2), (F16, 300, 2), (BF16, 300, 2)):
+        L, D = 400, 64
+        k, v = _rand((1, L, 1, D), dtype, 0), _rand((1, L, 1, D), dtype, 1)
+        k2, v2 = k.clone(), v.clone()
+        for t, bad in ((k2, float("inf")), (v2, float("nan"))):
+            t[:, -3:] = bad
+            t[:, -3:, :, ::2] = torch.finfo(dtype).min
+        q = _rand((1, Sq, H, D), dtype, 2).cuda()
+        outs = []
+        for a, b in ((k, v), (k2, v2)):
+            cache, table = PagedKVCache(26, 16, 1, D, dtype), _table(1, 25, 26, 0)
+            append_paged(cache, a.cuda(), b.cuda(), _i32(table), _i32([0]))
+            outs.append(attend_paged(q, cache, _i32(table), _i32([L])))
+        assert torch.equal(outs[0][:, :-3], outs[1][:, :-3])
+        assert torch.isfinite(outs[1][:, :-3]).all()
+
+
 def test_lengths_past_the_table_and_many_sequences():
     from flash_attn_volta import attend_paged
     B = 150                                                # over two scans of 64
