@@ -196,12 +196,13 @@ int launch_read_d(const fa::ReadArgs &a, int D, hipStream_t st) {
 struct AttnPlan {
   int nt, row_tiles, target, slots;
   int64_t rows;
-  // partial results: none where no sequence is split
+  // partial results of the chunks of split sequences (fa::find_chunk): 68 MiB at
+  // most on 256 compute units
   size_t o_bytes(int Hk, int D) const {
-    return target > 1 ? (size_t)slots * Hk * rows * D * sizeof(float) : 0;
+    return target > 1 ? (size_t)(target + 1) * Hk * rows * D * sizeof(float) : 0;
   }
   size_t bytes(int Hk, int D) const {
-    return target > 1 ? o_bytes(Hk, D) + (size_t)slots * Hk * rows * 2 * sizeof(float) : 0;
+    return target > 1 ? o_bytes(Hk, D) + (size_t)(target + 1) * Hk * rows * 2 * sizeof(float) : 0;
   }
 };
 
@@ -438,7 +439,6 @@ int fa_paged_attn(const void *q, const fa_paged_cache *cache, const int32_t *tab
   a.Sq = Sq;
   a.H = H;
   a.G = H / Hk;
-  a.slots = p.slots;
   a.target = p.target;
   // never 0, so that masked (-inf) scores stay -inf
   a.c = fmaxf(fabsf(sm_scale) * fa::kLog2e, 1e-30f);

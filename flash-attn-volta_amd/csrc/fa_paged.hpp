@@ -322,10 +322,9 @@ struct PagedAttnArgs {
   f16 *o;                               // (B, Sq, H, D) contiguous
   float *lse;                           // (B, H, Sq) or NULL
   const int32_t *lengths, *counts;      // counts: NULL = Sq everywhere
-  float *part_o;                        // (slots, Hk, rows, D) unnormalised
-  float *part_ml;                       // (slots, Hk, rows, 2): maximum (log2), sum
+  float *part_o;                        // (target + 1, Hk, rows, D) unnormalised
+  float *part_ml;                       // (target + 1, Hk, rows, 2): maximum (log2), sum
   int B, Sq, H, G;
-  int slots;                            // chunks in all, at most
   int target;                           // chunks aimed at
   float c;                              // |sm_scale| log2 e
   uint32_t flip;                        // sign bits xor-ed into q (negative scale)
@@ -338,7 +337,7 @@ constexpr float kLowest = -3.4028234663852886e38f;
 
 struct Chunk {
   int b, index, count, keys;            // `count` chunks of `keys` keys in sequence b
-  int first;                            // slot of the sequence's chunk 0
+  int part;                             // partial result of its chunk 0, where count > 1
   int length, held;                     // lengths[b], and what of it the table holds
 };
 
@@ -368,8 +367,10 @@ __device__ __forceinline__ int wave_prefix(int x) {
 // whatever the lengths.  The host knows no lengths; every wave counts them for
 // itself (B loads) and finds the sequence of its slot; one that holds nothing is
 // a chunk too, which writes its zeros.  max(target, (target + 1) / 2 + B) slots
-// cover every chunk, B with a target of 1 (then no sequence is split).  With
-// `by_sequence` the argument is a sequence and its chunks are returned.
+// cover every chunk, B with a target of 1 (then no sequence is split); those of
+// sequences that are split are target + 1 at most (n > 1 chunks are under twice
+// their units' share).  With `by_sequence` the argument is a sequence and its
+// chunks are returned.
 __device__ __forceinline__ bool find_chunk(const PagedAttnArgs &a, int want, bool by_sequence,
                                            Chunk &out) {
   const int lane = threadIdx.x & 63;
@@ -384,7 +385,7 @@ __device__ __forceinline__ bool find_chunk(const PagedAttnArgs &a, int want, boo
     return max(1, q);
   };
   if (a.B == 1) {                       // one user's tokens: scalar work alone
-    out.b = out.first = 0;
+    out.b = out.part = 0;
     out.length = a.lengths[0];
     out.held = held_keys(a, out.length);
     const int u = units_of(out.held), units = parts(u, a.target);
@@ -404,17 +405,21 @@ __device__ __forceinline__ bool find_chunk(const PagedAttnArgs &a, int want, boo
     held = held_keys(a, length);
     return units_of(held);
   };
-  auto find = [&](int first, int n, int b0, int units) {
+  // Prefix sums of the chunks and of those of split sequences: two 16-bit halves,
+  // under 2^15 both (targets are workgroups of one round, 64 sequences a time).
+  auto prefix = [&](int n) { return wave_prefix(n | (n > 1 ? n << 16 : 0)); };
+  auto find = [&](int upto, int n, int b0, int before, int before_split, int units) {
+    const int first = before + (upto & 0xFFFF) - n;
     const bool mine = by_sequence ? b0 + lane == want : (want >= first && want < first + n);
     const uint64_t hit = __ballot(mine);
     if (!hit) return false;
     const int src = __builtin_ctzll(hit);
     out.b = b0 + src;
-    out.first = __builtin_amdgcn_readlane(first, src);
     out.count = __builtin_amdgcn_readlane(n, src);
+    out.part = before_split + __builtin_amdgcn_readlane((upto >> 16) - n, src);
     out.length = __builtin_amdgcn_readlane(length, src);
     out.held = __builtin_amdgcn_readlane(held, src);
-    out.index = want - out.first;
+    out.index = want - __builtin_amdgcn_readlane(first, src);
     out.keys = units * kUnit;
     return true;
   };
@@ -422,13 +427,13 @@ __device__ __forceinline__ bool find_chunk(const PagedAttnArgs &a, int want, boo
   if (a.B <= 64) {
     const int u = load(lane), total = last(wave_prefix(u));
     int units = max(1, (total + a.target - 1) / a.target);
-    int n = lane < a.B ? parts(u, units) : 0, upto = wave_prefix(n);
-    if (last(upto) > a.target) {
+    int n = lane < a.B ? parts(u, units) : 0, upto = prefix(n);
+    if ((last(upto) & 0xFFFF) > a.target) {
       units = fewer(total);
       n = lane < a.B ? parts(u, units) : 0;
-      upto = wave_prefix(n);
+      upto = prefix(n);
     }
-    return find(upto - n, n, 0, units);
+    return find(upto, n, 0, 0, 0, units);
   }
   auto sum = [&](auto &&f) {            // over all sequences
     int x = 0;
@@ -441,12 +446,13 @@ __device__ __forceinline__ bool find_chunk(const PagedAttnArgs &a, int want, boo
   const int total = sum([](int u) { return u; });
   int units = max(1, (total + a.target - 1) / a.target);
   if (sum([&](int u) { return parts(u, units); }) > a.target) units = fewer(total);
-  int before = 0;
+  int before = 0, before_split = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
     const int u = load(b0 + lane), n = b0 + lane < a.B ? parts(u, units) : 0;
-    const int upto = wave_prefix(n);
-    if (find(before + upto - n, n, b0, units)) return true;
-    before += last(upto);
+    const int upto = prefix(n);
+    if (find(upto, n, b0, before, before_split, units)) return true;
+    before += last(upto) & 0xFFFF;
+    before_split += last(upto) >> 16;
   }
   return false;
 }
@@ -706,7 +712,7 @@ __global__ __launch_bounds__(256) void fa_paged_few_kernel(PagedAttnArgs a) {
   }
   const bool real = i < count, whole = ch.count == 1;
   const float inv = !real || sum == 0.0f ? 0.0f : (whole ? 1.0f / sum : 1.0f);   // (NaN: kept)
-  const int64_t part = ((int64_t)slot * Hk + hk) * rows + row;
+  const int64_t part = ((int64_t)(ch.part + ch.index) * Hk + hk) * rows + row;
   const int64_t out = (((int64_t)b * a.Sq + i) * a.H + h) * D;
   for (int d = tid % lanes; d < D; d += lanes) {
     float acc = 0.0f;
@@ -927,7 +933,7 @@ __global__ __launch_bounds__(256, 2) void fa_paged_rows_kernel(PagedAttnArgs a) 
   const bool seen = real && l != 0.0f;                  // (NaN counts as seen)
   const bool whole = ch.count == 1;
   const float f = whole ? (seen ? 1.0f / l : 0.0f) : (real ? 1.0f : 0.0f);
-  const int64_t part = ((int64_t)slot * Hk + hk) * rows + row;
+  const int64_t part = ((int64_t)(ch.part + ch.index) * Hk + hk) * rows + row;
   E *out = reinterpret_cast<E *>(a.o) + (((int64_t)b * a.Sq + qi) * a.H + h) * D;
   // registers j and j + 8 of every dt are 2 ND consecutive columns
 #pragma unroll
@@ -981,7 +987,7 @@ __global__ __launch_bounds__(256) void fa_paged_merge_kernel(PagedAttnArgs a) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int k = min(k0 + j * NS, ch.count - 1);
-      const int64_t p = ((int64_t)(ch.first + k) * Hk + hk) * rows + row;
+      const int64_t p = ((int64_t)(ch.part + k) * Hk + hk) * rows + row;
       const floatx2 ml = *reinterpret_cast<const floatx2 *>(a.part_ml + p * 2);
       mk[j] = ml[0];
       lk[j] = ml[1];

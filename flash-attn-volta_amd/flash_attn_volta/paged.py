@@ -61,8 +61,7 @@ class PagedKVCache:
     append_paged and must not be put there.
     """
 
-    __slots__ = ("_tensors", "dtype", "num_pages", "page_size", "num_kv_heads", "head_dim", "device",
-                 "_structs", "_addrs", "_half", "_like")
+    __slots__ = ("_tensors", "_dtype", "_sizes", "_structs", "_half", "_like", "_head_dim")
 
     def __init__(self, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int,
                  dtype: torch.dtype = torch.bfloat16, device="cuda"):
@@ -105,46 +104,39 @@ class PagedKVCache:
             _require(t.device == codes.device, "the cache's tensors must be on one device")
             _require(t.is_contiguous() and t.data_ptr() % 16 == 0,
                      lambda: f"{name} must be contiguous and 16-byte aligned")
-        # (kept as they are: the calls' structs hold their addresses)
-        self._tensors, self._like = dict(tensors), codes
-        self.dtype, self.device = dtype, codes.device
-        self.num_pages, self.num_kv_heads, self.page_size, self.head_dim = N, H, P, D
-        self._structs, self._addrs, self._half = {}, {}, dtype == torch.float16
+        # (fixed from here on: the calls' structs hold addresses and sizes)
+        self._tensors, self._like, self._dtype = dict(tensors), codes, dtype
+        self._sizes, self._head_dim = (N, H, P), D
+        self._structs, self._half = {}, dtype == torch.float16
 
     k_codes = property(lambda self: self._tensors["k_codes"])
     k_scales = property(lambda self: self._tensors["k_scales"])
     v_codes = property(lambda self: self._tensors["v_codes"])
     v_scales = property(lambda self: self._tensors["v_scales"])
+    num_pages = property(lambda self: self._sizes[0])
+    num_kv_heads = property(lambda self: self._sizes[1])
+    page_size = property(lambda self: self._sizes[2])
+    head_dim = property(lambda self: self._head_dim)
+    dtype = property(lambda self: self._dtype)
+    device = property(lambda self: self._like.device)
 
     @property
     def nbytes(self) -> int:
         return sum(t.numel() for t in self._tensors.values())
 
+    def __reduce__(self):               # copies and pickles: their own addresses
+        return PagedKVCache.from_tensors, (self.k_codes, self.k_scales, self.v_codes,
+                                           self.v_scales, self.dtype)
+
     def _struct(self, width: int):
-        """fa_paged_cache for a table of `width` pages a sequence."""
+        """(fa_paged_cache for a table of `width` pages a sequence, its address)."""
         s = self._structs.get(width)
         if s is None:
-            if len(self._structs) >= 64:
-                self._structs.clear()
-            s = self._structs[width] = _capi.PagedCacheStruct(
+            c = _capi.PagedCacheStruct(
                 self.k_codes.data_ptr(), self.k_scales.data_ptr(), self.v_codes.data_ptr(),
                 self.v_scales.data_ptr(), self.num_pages, self.page_size, self.num_kv_heads, width)
+            s = self._structs[width] = (c, ctypes.addressof(c))
         return s
-
-    def _addr(self, table) -> int:
-        """Address of _struct(width of `table`); 0 where that is no table."""
-        if not isinstance(table, torch.Tensor) or table.dim() != 2 or table.shape[1] == 0:
-            return 0
-        width = table.shape[1]
-        a = self._addrs.get(width)
-        if a is None:
-            s = self._struct(width)
-            if len(self._addrs) >= 64:
-                self._addrs.clear()
-            a, _ = self._addrs[width] = (ctypes.addressof(s), s)
-        else:
-            a = a[0]
-        return a
 
     def __repr__(self):
         return (f"PagedKVCache({self.num_pages} pages of {self.page_size} tokens, "
@@ -205,7 +197,9 @@ def _fast(cache, page_table, *tensors) -> int:
     for t in tensors:
         if not isinstance(t, torch.Tensor):
             return 0
-    return cache._addr(page_table)
+    if not isinstance(page_table, torch.Tensor) or page_table.dim() != 2 or page_table.shape[1] == 0:
+        return 0
+    return cache._struct(page_table.shape[1])[1]
 
 
 def append_paged(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor,
@@ -240,9 +234,8 @@ def append_paged(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, page_tab
             and (counts is None or isinstance(counts, torch.Tensor)) \
             and (rotary is None or isinstance(rotary, RotaryPositions)):
         done, out = _cpp.paged_append(
-            addr, cache._like, cache._half, cache.head_dim, page_table, k, v, q, start, counts,
-            *((None, 1.0, 0, 0) if rotary is None else
-              (rotary.steps, rotary.attention_factor, rotary.rotary_dim, rotary._flags)))
+            addr, cache._like, cache._half, cache._head_dim, page_table, k, v, q, start, counts,
+            *((None, 1.0, 0, 0) if rotary is None else rotary._args))
         if done:
             return out
     _require(isinstance(k, torch.Tensor), "k must be a tensor")
@@ -277,7 +270,7 @@ def append_paged(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, page_tab
     lib = _capi.load()
     with _on_device(k.device):
         rc = lib.fa_paged_append(
-            cache._struct(page_table.shape[1]), page_table.data_ptr(), page_table.stride(0),
+            cache._struct(page_table.shape[1])[0], page_table.data_ptr(), page_table.stride(0),
             k.data_ptr(), v.data_ptr(), q.data_ptr() if rows else None, _ptr(q_out) if rows else None,
             start.data_ptr(), _ptr(counts), steps, factor, R, flags, B, S, H, D,
             kernel_strides(k), kernel_strides(v), kernel_strides(q) if rows else None,
@@ -294,7 +287,7 @@ def read_paged(cache: PagedKVCache, page_table: torch.Tensor, start: torch.Tenso
     For moving a sequence, a dense prefill over its prefix, or inspection."""
     addr = _fast(cache, page_table, start)
     if addr and isinstance(length, int) and (counts is None or isinstance(counts, torch.Tensor)):
-        out = _cpp.paged_read(addr, cache._like, cache._half, cache.head_dim, page_table, start,
+        out = _cpp.paged_read(addr, cache._like, cache._half, cache._head_dim, page_table, start,
                               length, counts)
         if out is not None:
             return out
@@ -315,7 +308,7 @@ def read_paged(cache: PagedKVCache, page_table: torch.Tensor, start: torch.Tenso
     lib = _capi.load()
     with _on_device(cache.device):
         rc = lib.fa_paged_read(
-            cache._struct(page_table.shape[1]), page_table.data_ptr(), page_table.stride(0),
+            cache._struct(page_table.shape[1])[0], page_table.data_ptr(), page_table.stride(0),
             k.data_ptr(), v.data_ptr(), start.data_ptr(), _ptr(counts), B, length, D,
             _DTYPES[cache.dtype], _stream_ptr(cache.device))
     _capi.check(rc, "fa_paged_read")
@@ -359,8 +352,8 @@ def attend_paged(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tensor,
     addr = _fast(cache, page_table, q, lengths)
     if addr and (counts is None or isinstance(counts, torch.Tensor)):
         out = _cpp.paged_attend(
-            addr, cache._like, cache._half, cache.head_dim, q, page_table, lengths, counts,
-            cache.head_dim ** -0.5 if sm_scale is None else float(sm_scale),
+            addr, cache._like, cache._half, cache._head_dim, q, page_table, lengths, counts,
+            cache._head_dim ** -0.5 if sm_scale is None else float(sm_scale),
             bool(return_softmax_lse))
         if out is not None:
             return out if return_softmax_lse else out[0]
@@ -387,7 +380,7 @@ def attend_paged(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tensor,
         nbytes = _ws_bytes(lib, B, Sq, H, Hk, D)
         ws = _runtime.workspace(nbytes, q.device, stream) if nbytes else None
         rc = lib.fa_paged_attn(
-            q.data_ptr(), cache._struct(page_table.shape[1]), page_table.data_ptr(),
+            q.data_ptr(), cache._struct(page_table.shape[1])[0], page_table.data_ptr(),
             page_table.stride(0), lengths.data_ptr(), _ptr(counts), out.data_ptr(), _ptr(lse),
             _ptr(ws), nbytes, B, Sq, H, D, kernel_strides(q), float(sm_scale),
             _DTYPES[cache.dtype], stream)

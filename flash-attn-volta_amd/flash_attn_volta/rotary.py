@@ -124,7 +124,7 @@ class RotaryPositions:
     floats, radians a position), steps (the device tensor the kernels read).
     """
 
-    __slots__ = ("rotary_dim", "interleaved", "attention_factor", "frequencies", "steps", "_flags")
+    __slots__ = ("_args", "_frequencies")
 
     def __init__(self, rotary_dim: int, base: float = 10000.0, *, interleaved: bool = False,
                  scaling: dict | None = None, device="cuda"):
@@ -132,14 +132,19 @@ class RotaryPositions:
                  lambda: f"rotary_dim must be an even number from 2 to 256, got {rotary_dim!r}")
         _require(isinstance(base, (int, float)) and math.isfinite(base) and base > 0,
                  lambda: f"base must be a positive number, got {base!r}")
-        self.rotary_dim = rotary_dim
-        self.interleaved = bool(interleaved)
-        self.frequencies, self.attention_factor = _scaled_frequencies(rotary_dim, float(base),
-                                                                      scaling)
-        steps = [round(Fraction(f) * (1 << 64) / _TWO_PI) % (1 << 64) for f in self.frequencies]
-        self.steps = torch.tensor([s - (1 << 64) if s >> 63 else s for s in steps],
-                                  dtype=torch.int64, device=device)
-        self._flags = _capi.FA_ROTARY_INTERLEAVED if self.interleaved else 0
+        self._frequencies, factor = _scaled_frequencies(rotary_dim, float(base), scaling)
+        steps = [round(Fraction(f) * (1 << 64) / _TWO_PI) % (1 << 64) for f in self._frequencies]
+        steps = torch.tensor([s - (1 << 64) if s >> 63 else s for s in steps], dtype=torch.int64,
+                             device=device)
+        # (fixed: the kernels read rotary_dim / 2 steps)
+        self._args = (steps, factor, rotary_dim, _capi.FA_ROTARY_INTERLEAVED if interleaved else 0)
+
+    steps = property(lambda self: self._args[0])
+    attention_factor = property(lambda self: self._args[1])
+    rotary_dim = property(lambda self: self._args[2])
+    interleaved = property(lambda self: bool(self._args[3]))
+    frequencies = property(lambda self: list(self._frequencies))
+    _flags = property(lambda self: self._args[3])
 
     def __repr__(self):
         return (f"RotaryPositions(rotary_dim={self.rotary_dim}, interleaved={self.interleaved}, "
@@ -274,8 +279,7 @@ def apply_rotary_positions(q: torch.Tensor, k: torch.Tensor | None, positions: t
     if _cpp is not None and isinstance(rotary, RotaryPositions) and not _transforms_active() \
             and not _compiling() and all(isinstance(t, torch.Tensor) for t in (q, positions)) \
             and (k is None or isinstance(k, torch.Tensor)):
-        out = _cpp.rotary(q, k, positions, rotary.steps, rotary.attention_factor,
-                          rotary.rotary_dim, rotary._flags)
+        out = _cpp.rotary(q, k, positions, *rotary._args)
         if out is not None:
             return out
     _check(q, k, rotary)

@@ -195,3 +195,27 @@ def test_no_cpu_path():
                  lambda: apply_rotary_positions(k, None, n, RotaryPositions(32, device="cpu"))):
         with pytest.raises(FlashAttnArgumentError):
             call()
+
+
+def test_handles_are_fixed_and_copy():
+    """What the kernels are given sizes of cannot be exchanged under them; copies have
+    tensors of their own."""
+    import copy
+    import pickle
+    from flash_attn_volta import PagedKVCache, RotaryPositions
+    cache = PagedKVCache(2, 16, 1, 32, torch.float16, device="cpu")
+    rot = RotaryPositions(32, device="cpu")
+    for obj, names in ((cache, ("k_codes", "head_dim", "num_pages", "dtype", "page_size")),
+                       (rot, ("steps", "rotary_dim", "attention_factor", "interleaved"))):
+        for n in names:
+            with pytest.raises(AttributeError):
+                setattr(obj, n, getattr(obj, n))
+    cache._struct(3)
+    other = copy.deepcopy(cache)
+    assert other.k_codes.data_ptr() != cache.k_codes.data_ptr() and other.dtype == torch.float16
+    assert other._struct(3)[0].k_codes == other.k_codes.data_ptr()
+    again = pickle.loads(pickle.dumps(cache))
+    assert again.num_pages == 2 and again.head_dim == 32 and torch.equal(again.v_codes, cache.v_codes)
+    assert copy.copy(rot).steps is rot.steps and copy.deepcopy(rot).frequencies == rot.frequencies
+    rot.frequencies.clear()
+    assert len(rot.frequencies) == 16

@@ -81,6 +81,31 @@ def test_forward_and_backward(B, S, H, Hk, D, R, inter, scaling, dtype, first, l
         _check(got.detach(), x, pos, rot, inverse, what)
 
 
+@pytest.mark.parametrize("D,R,inter", [(24, 16, True), (24, 24, False), (40, 32, False), (40, 8, False),
+                                       (48, 48, False), (96, 64, True), (80, 18, False)])
+def test_other_head_dims(D, R, inter):
+    from flash_attn_volta import RotaryPositions, apply_rotary_positions
+    rot = RotaryPositions(R, interleaved=inter)
+    x = _inputs(2, 11, 3, D, torch.float16, D)
+    pos = 40 + np.arange(11)[None] + np.zeros((2, 1), dtype=np.int64)
+    got = apply_rotary_positions(x.cuda(), None, torch.arange(40, 51, device="cuda"), rot)[0]
+    _check(got, x, pos, rot, False, "x")
+
+
+def test_gradients_of_expanded_and_wide_upstreams():
+    """A sum's gradient (strides of 0) and an fp32 one are taken."""
+    from flash_attn_volta import RotaryPositions, apply_rotary_positions, rotary_backward
+    rot = RotaryPositions(64)
+    pos = torch.arange(5, device="cuda")
+    x = _inputs(1, 5, 2, 64, torch.float16, 0).cuda().requires_grad_()
+    apply_rotary_positions(x, None, pos, rot)[0].sum().backward()
+    want = rotary_backward(torch.ones_like(x), None, pos, rot)[0]
+    assert torch.equal(x.grad, want)
+    x.grad = None
+    apply_rotary_positions(x, None, pos, rot)[0].float().sum().backward()
+    assert torch.equal(x.grad, want)
+
+
 def test_gradient_against_differences():
     """The map is linear: f(x + h e) - f(x) = h f(e) for any step h.  Powers of
     two and inputs of few bits make x + h e exact; each f is off by half a step
