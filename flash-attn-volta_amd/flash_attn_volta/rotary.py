@@ -35,8 +35,16 @@ from .forward import (FlashAttnArgumentError, _DTYPES, _kernel_ready, _on_device
 
 __all__ = ["RotaryPositions", "apply_rotary_positions", "rotary_forward", "rotary_backward"]
 
-# 2 pi to 50 digits: a step is exact to 2^-64 turns whatever the frequency
-_TWO_PI = Fraction("6.28318530717958647692528676655900576839433879875021")
+# 2^64 / (2 pi) in units of 2^-80 (2 pi to 50 digits): a step is exact to 2^-64
+# turns whatever the frequency
+_TURN = round(Fraction(1 << 144) / Fraction("6.28318530717958647692528676655900576839433879875021"))
+
+
+def _step(f: float) -> int:
+    """f / (2 pi) turns a position, mod 1 in units of 2^-64, as an int64."""
+    n, d = f.as_integer_ratio()
+    s = ((n * _TURN // d + (1 << 79)) >> 80) % (1 << 64)
+    return s - (1 << 64) if s >> 63 else s
 
 
 def _number(scaling: dict, name: str, default=None) -> float:
@@ -133,9 +141,7 @@ class RotaryPositions:
         _require(isinstance(base, (int, float)) and math.isfinite(base) and base > 0,
                  lambda: f"base must be a positive number, got {base!r}")
         self._frequencies, factor = _scaled_frequencies(rotary_dim, float(base), scaling)
-        steps = [round(Fraction(f) * (1 << 64) / _TWO_PI) % (1 << 64) for f in self._frequencies]
-        steps = torch.tensor([s - (1 << 64) if s >> 63 else s for s in steps], dtype=torch.int64,
-                             device=device)
+        steps = torch.tensor([_step(f) for f in self._frequencies], dtype=torch.int64, device=device)
         # (fixed: the kernels read rotary_dim / 2 steps)
         self._args = (steps, factor, rotary_dim, _capi.FA_ROTARY_INTERLEAVED if interleaved else 0)
 
