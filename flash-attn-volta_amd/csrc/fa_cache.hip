@@ -225,6 +225,9 @@ AttnPlan attn_plan(int B, int Sq, int H, int Hk, int cus, int64_t capacity) {
   const int64_t resident = (int64_t)(p.nt == 1 ? 4 : 2) * cus / ((int64_t)Hk * p.row_tiles);
   p.target = resident < 1 || capacity <= fa::kUnit ? 1 : (int)resident;   // (a unit is never split)
   p.slots = p.target > 1 ? std::max(p.target, (p.target + 1) / 2 + B) : B;   // fa::find_chunk
+  // (no more than the units that the table holds)
+  const int64_t units = (std::min(capacity, (int64_t)1 << 30) + fa::kUnit - 1) / fa::kUnit;
+  p.slots = (int)std::min((int64_t)p.slots, units * B);
   return p;
 }
 

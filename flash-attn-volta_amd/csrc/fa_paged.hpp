@@ -116,7 +116,8 @@ __device__ __forceinline__ uint32_t quantise8(float *y, float top, int max_byte,
 // fp32, as fa_rotary does.  Consecutive lanes are the D/8 chunks of a key's
 // row, then the tokens, whose 4-byte pieces of an interleaved V group then fill
 // whole lines.  Bound by HBM on prompts and by launch and load latency on single
-// tokens.
+// tokens: 6001 tokens of 32 / 8 heads of 128 with q, 32.4 us, 4.0 TB/s (80 % of a
+// large copy's rate); one token 3.5 us.
 template <typename E, int D>
 __global__ __launch_bounds__(kAppendThreads) void fa_paged_append_kernel(AppendArgs a) {
   extern __shared__ char smem[];
@@ -263,7 +264,8 @@ struct ReadArgs {
 };
 
 // Tokens start[b] .. start[b] + n - 1 as 16-bit rows; 0 where nothing is held
-// (behind counts[b], outside the table, on a page that is none).
+// (behind counts[b], outside the table, on a page that is none).  Bound by HBM, by
+// what it writes: 6001 tokens of 8 heads of 128 8.2 us (3.8 TB/s).
 template <typename E, int D>
 __global__ __launch_bounds__(256) void fa_paged_read_kernel(ReadArgs a) {
   constexpr int NCH = D / 8;
@@ -556,6 +558,10 @@ __device__ __forceinline__ void pv_step(const Tile16<D> (&t)[2], const float (&v
 // bf16 probabilities go into the product as two bf16 numbers whose sum has 16
 // bits: the extra MFMAs hide behind the loads, and a single one would add a
 // rounding as large as the output's own.
+// 2 users' tokens on 131072 of 32 / 8 heads of 128: 51.6 us, 5.5 TB/s (a large copy
+// runs at 4.9); 32 on up to 3001: 15.7 us, 4.2 TB/s; one on 4096: 4.8 us, a launch
+// and three dependent loads (length, page, codes).  Vector instructions take 60 %
+// of the cycles, half of them conversions, matrix ones 12 %.
 template <typename E, int D, int NT>
 __global__ __launch_bounds__(256) void fa_paged_few_kernel(PagedAttnArgs a) {
   constexpr int KS = D / 32, ND = D / 16, NW = 4;
@@ -746,6 +752,11 @@ __global__ __launch_bounds__(256) void fa_paged_few_kernel(PagedAttnArgs a) {
 // the conversion of K of tile j + 2 and V of tile j + 1.
 // O^T tile dt, row 16 e + mm is column (D/16) mm + 2 dt + e: the order in which
 // code bytes give them.
+// 2048 queries of 32 / 8 heads of 128 on 8192 tokens: 240 us, 1.0 PFLOP/s, where a
+// large library product of this type reaches 1.2; matrix instructions busy 49 % of
+// the cycles, vector ones 59 %, at the 1.8 GHz that the card then runs at (842 us
+// by the few-row kernel; 258 us with the same conversion before the stages were
+// interleaved).  256 queries on 8448: 55 us.
 constexpr int kRowsTile = 128, kRowsKeys = 64;
 
 template <typename E, int D>
@@ -754,6 +765,8 @@ __global__ __launch_bounds__(256, 2) void fa_paged_rows_kernel(PagedAttnArgs a) 
   __shared__ u32x4 s_k[2][D / 8][kRowsKeys];
   __shared__ u32x4 s_v[2][kRowsKeys / 8][ND][32];      // [16-key part, h][dt][row]: 4 keys, +8
   __shared__ int s_hole[2][4];
+  static_assert(sizeof(s_k) >= 2 * 32 * D * sizeof(float) && sizeof(s_v) >= 2 * 32 * D * sizeof(float),
+                "the rows leave through both");
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int m = lane & 15, g = lane >> 4;              // as a converter
@@ -795,21 +808,23 @@ __global__ __launch_bounds__(256, 2) void fa_paged_rows_kernel(PagedAttnArgs a) 
 #pragma unroll
   for (int t = 0; t < ND; ++t) o[t] = floatx16{};
 
-  Tile16<D> raw;                        // K of the tile to convert, V of the one before it
-  int64_t v_row = 0;                    // where that V is, until it is loaded
-  auto load_keys = [&](int key) {
-    const int64_t r = tile_row(a.cache, b, hk, key + 16 * w, end, raw.hole);
-    load_k<D>(a.cache, r, m, g, raw);
-    return r;
+  // Codes in flight, for the next step and the one after it: K of a tile and V of
+  // the one before it (whose row is kept until then).
+  Tile16<D> raw0, raw1;
+  int64_t v_row = 0;
+  auto load = [&](int key, Tile16<D> &raw) {
+    load_v<D>(a.cache, v_row, m, g, raw);
+    v_row = tile_row(a.cache, b, hk, key + 16 * w, end, raw.hole);
+    load_k<D>(a.cache, v_row, m, g, raw);
   };
   // pieces of a tile's conversion: K chunk t of this lane's quarter of the
   // columns; columns 2t, 2t + 1 of this lane's V unit
-  auto convert_k = [&](int buf, auto T) {
+  auto convert_k = [&](int buf, const Tile16<D> &raw, auto T) {
     constexpr int t = decltype(T)::value;
     s_k[buf][ND * g + t][16 * w + m] = fp4_row8<E>(raw_word<D>(raw.k, t), fp4_scale(raw.ks));
     if constexpr (t == 0) s_hole[buf][w] = raw.hole;    // (every lane the same)
   };
-  auto convert_v = [&](int buf, auto T) {
+  auto convert_v = [&](int buf, const Tile16<D> &raw, auto T) {
     constexpr int t = decltype(T)::value;
     uint32_t x[4];
 #pragma unroll
@@ -825,10 +840,6 @@ __global__ __launch_bounds__(256, 2) void fa_paged_rows_kernel(PagedAttnArgs a) 
                                                false, false);
     s_v[buf][2 * w + (g & 1)][t][16 * hf + m] = u32x4{x0[0], x1[0], x0[1], x1[1]};
   };
-  auto convert = [&](int kbuf, int vbuf) {
-    static_for<ND>([&](auto T) { convert_k(kbuf, T); });
-    static_for<ND>([&](auto T) { convert_v(vbuf, T); });
-  };
   auto k_frag = [&](int buf, int i) {   // of score instruction i: columns i / 2, keys i % 2
     return __builtin_bit_cast(vec8<E>, s_k[buf][2 * (i >> 1) + hf][32 * (i & 1) + n]);
   };
@@ -837,16 +848,20 @@ __global__ __launch_bounds__(256, 2) void fa_paged_rows_kernel(PagedAttnArgs a) 
   };
   // masks tile `key`'s scores, and moves the running maximum where they leave the
   // old one behind by 2^8
+  const int lim = min(last, end - 1);   // the last position that this lane's row sees here
   auto settle = [&](int key, int buf, floatx16 (&x)[2]) {
-    const int holes = s_hole[buf][0] | s_hole[buf][1] | s_hole[buf][2] | s_hole[buf][3];
-    if (key + kRowsKeys > all || key + kRowsKeys > end || __builtin_amdgcn_readfirstlane(holes)) {
+    if (key + kRowsKeys > all || key + kRowsKeys > end) {
+      const int seen = lim - key - 4 * hf;
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
+      for (int i = 0; i < 32; ++i)
+        x[i >> 4][i & 15] = 32 * (i >> 4) + c_row(i & 15, 0) > seen ? kNegInf : x[i >> 4][i & 15];
+    }
+    int hole[4];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int kk = key + 32 * kt + c_row(i, hf);
-          if (kk > last || kk >= end || s_hole[buf][2 * kt + i / 8]) x[kt][i] = kNegInf;
-        }
+    for (int i = 0; i < 4; ++i) hole[i] = __builtin_amdgcn_readfirstlane(s_hole[buf][i]);
+    if (hole[0] | hole[1] | hole[2] | hole[3]) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) x[i >> 4][i & 15] = hole[i >> 3] ? kNegInf : x[i >> 4][i & 15];
     }
     float top = x[0][0];
 #pragma unroll
@@ -862,33 +877,19 @@ __global__ __launch_bounds__(256, 2) void fa_paged_rows_kernel(PagedAttnArgs a) 
     }
   };
 
-  if (key0 < end) {
-    // K of tiles 0 and 1, V of tile 0 converted; K of tile 2 and V of tile 1 loaded
-    int64_t r = load_keys(key0);
-    load_v<D>(a.cache, r, m, g, raw);
-    convert(0, 0);
-    r = load_keys(key0 + kRowsKeys);
-    static_for<ND>([&](auto T) { convert_k(1, T); });
-    load_v<D>(a.cache, r, m, g, raw);
-    v_row = load_keys(key0 + 2 * kRowsKeys);
-  }
-  __syncthreads();
-  if (key0 < wend) {
-    s[0] = s[1] = floatx16{};
-#pragma unroll
-    for (int i = 0; i < 2 * NS; ++i) s[i & 1] = mfma32(k_frag(0, i), qf[i >> 1], s[i & 1]);
-    settle(key0, 0, s);
-  }
-  __syncthreads();                      // K of tile 0 is overwritten next
-  int buf = 0;
-  for (int key = key0; key < end; key += kRowsKeys, buf ^= 1) {
-    if (key < wend) {
+  // Step `key` multiplies tile `key`, takes the scores of the next one, converts K of
+  // the one after that and V of the next, and loads what is converted two steps
+  // on; two steps before the first tile fill the pipeline.
+  auto sweep = [&](int key, Tile16<D> &raw, auto Buf) {
+    constexpr int buf = decltype(Buf)::value;
+    const bool more = key + kRowsKeys >= key0 && key + kRowsKeys < wend;
+    floatx16 next[2];
+    next[0] = next[1] = floatx16{};
+    if (key >= key0 && key < wend) {
       // The order is fixed here: fragments are read kAhead instructions before
       // the matrix instruction that takes them, and each of those is followed
       // by its share of the other work, which runs beside it.
       constexpr int kAhead = 4, kScore = 2 * NS, kProd = 4 * ND;
-      floatx16 next[2];
-      next[0] = next[1] = floatx16{};
       vec8<E> p[4], kf[kScore], vf[kProd];
       static_for<kAhead>([&](auto I) { kf[I] = k_frag(buf ^ 1, I); });
       static_for<kScore>([&](auto I) {
@@ -910,54 +911,85 @@ __global__ __launch_bounds__(256, 2) void fa_paged_rows_kernel(PagedAttnArgs a) 
         constexpr int i = decltype(I)::value;
         if constexpr (i + kAhead < kProd) vf[i + kAhead] = v_frag(buf, i + kAhead);
         o[i % ND] = mfma32(vf[i], p[i / ND], o[i % ND]);
-        if constexpr (i % 2 == 1 && i < 2 * ND) convert_k(buf, std::integral_constant<int, i / 2>{});
+        if constexpr (i % 2 == 1 && i < 2 * ND)
+          convert_k(buf, raw, std::integral_constant<int, i / 2>{});
         if constexpr (i % 2 == 1 && i >= 2 * ND)
-          convert_v(buf ^ 1, std::integral_constant<int, i / 2 - ND>{});
+          convert_v(buf ^ 1, raw, std::integral_constant<int, i / 2 - ND>{});
         __builtin_amdgcn_sched_barrier(0);
       });
-      load_v<D>(a.cache, v_row, m, g, raw);
-      v_row = load_keys(key + 3 * kRowsKeys);
-      s[0] = next[0];
-      s[1] = next[1];
-      if (key + kRowsKeys < wend) settle(key + kRowsKeys, buf ^ 1, s);
     } else {
-      convert(buf, buf ^ 1);
-      load_v<D>(a.cache, v_row, m, g, raw);
-      v_row = load_keys(key + 3 * kRowsKeys);
+      if (more) {
+#pragma unroll
+        for (int i = 0; i < 2 * NS; ++i)
+          next[i & 1] = mfma32(k_frag(buf ^ 1, i), qf[i >> 1], next[i & 1]);
+      }
+      static_for<ND>([&](auto T) { convert_k(buf, raw, T); });
+      static_for<ND>([&](auto T) { convert_v(buf ^ 1, raw, T); });
     }
+    load(key + 4 * kRowsKeys, raw);
+    s[0] = next[0];
+    s[1] = next[1];
+    if (more) settle(key + kRowsKeys, buf ^ 1, s);
     __syncthreads();
+  };
+  if (key0 < end) {
+    v_row = tile_row(a.cache, b, hk, key0 + 16 * w, end, raw0.hole);
+    load_k<D>(a.cache, v_row, m, g, raw0);
+    raw0.v = KRaw<D>{};
+    raw0.vs = 0;
+    load(key0 + kRowsKeys, raw1);
+    for (int key = key0 - 2 * kRowsKeys; key < end; key += 2 * kRowsKeys) {
+      sweep(key, raw0, std::integral_constant<int, 0>{});
+      if (key + kRowsKeys < end) sweep(key + kRowsKeys, raw1, std::integral_constant<int, 1>{});
+    }
   }
 
-  if (row >= rows) return;
+  // Rows leave through LDS: a lane holds 8 pieces of 2 ND columns of one row, and
+  // stores of those would each touch as many lines as lanes (7000 cycles of a
+  // workgroup, a third of a short sweep).  Piece mm of row n is kept at mm ^ n % 16.
   l += xor32(l);
-  const bool seen = real && l != 0.0f;                  // (NaN counts as seen)
   const bool whole = ch.count == 1;
+  const bool seen = real && l != 0.0f;                  // (NaN counts as seen)
   const float f = whole ? (seen ? 1.0f / l : 0.0f) : (real ? 1.0f : 0.0f);
-  const int64_t part = ((int64_t)(ch.part + ch.index) * Hk + hk) * rows + row;
-  E *out = reinterpret_cast<E *>(a.o) + (((int64_t)b * a.Sq + qi) * a.H + h) * D;
-  // registers j and j + 8 of every dt are 2 ND consecutive columns
+  const int64_t part = ((int64_t)(ch.part + ch.index) * Hk + hk) * rows;
+  auto leave = [&](auto *kept, auto &&place) {          // kept: 32 rows of this wave in LDS
+    typedef std::remove_reference_t<decltype(*kept)> X;
+    constexpr int kPiece = 2 * ND;
+    typedef X Piece __attribute__((ext_vector_type(kPiece)));
+    Piece *mine = reinterpret_cast<Piece *>(kept);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int d = NS * c_row(j, hf);
-    float x[2 * ND];
+    for (int j = 0; j < 8; ++j) {
+      Piece x;
 #pragma unroll
-    for (int t = 0; t < ND; ++t) {
-      x[2 * t] = seen || !whole ? o[t][j] * f : 0.0f;
-      x[2 * t + 1] = seen || !whole ? o[t][j + 8] * f : 0.0f;
+      for (int t = 0; t < ND; ++t) {
+        x[2 * t] = (X)(f == 0.0f ? 0.0f : o[t][j] * f);
+        x[2 * t + 1] = (X)(f == 0.0f ? 0.0f : o[t][j + 8] * f);
+      }
+      mine[n * 16 + (c_row(j, hf) ^ (n & 15))] = x;
     }
-    if (whole) {
-      E y[2 * ND];
+    // (a wave reads back its own rows: no barrier)
 #pragma unroll
-      for (int t = 0; t < 2 * ND; ++t) y[t] = (E)x[t];
-      __builtin_memcpy(__builtin_assume_aligned(out + d, 4 * ND), y, sizeof y);
-    } else {
-      __builtin_memcpy(__builtin_assume_aligned(a.part_o + part * D + d, 8 * ND), x, sizeof x);
+    for (int j = 0; j < 8; ++j) {
+      const int at = 64 * j + lane, r = at >> 4, mm = at & 15, out_row = row0 + 32 * w + r;
+      if (out_row < rows)
+        *reinterpret_cast<Piece *>(place(out_row) + kPiece * mm) = mine[r * 16 + (mm ^ (r & 15))];
     }
+  };
+  if (whole) {
+    leave(reinterpret_cast<E *>(&s_k[0][0][0]) + w * 32 * D, [&](int r) {
+      const int i = r / a.G;
+      return reinterpret_cast<E *>(a.o) +
+             (((int64_t)b * a.Sq + i) * a.H + hk * a.G + (r - i * a.G)) * D;
+    });
+  } else {                              // two waves' fp32 rows fill s_k, two s_v
+    float *half = w < 2 ? reinterpret_cast<float *>(&s_k[0][0][0])
+                        : reinterpret_cast<float *>(&s_v[0][0][0][0]);
+    leave(half + (w & 1) * 32 * D, [&](int r) { return a.part_o + (part + r) * D; });
   }
-  if (hf != 0) return;
+  if (hf != 0 || row >= rows) return;
   if (!whole) {
-    a.part_ml[part * 2] = mx;
-    a.part_ml[part * 2 + 1] = real ? l : 0.0f;
+    a.part_ml[(part + row) * 2] = mx;
+    a.part_ml[(part + row) * 2 + 1] = real ? l : 0.0f;
   } else if (a.lse) {
     a.lse[((int64_t)b * a.H + h) * a.Sq + qi] = seen ? (mx + fast_log2(l)) * kLn2 : kPosInf;
   }
@@ -966,7 +998,8 @@ __global__ __launch_bounds__(256, 2) void fa_paged_rows_kernel(PagedAttnArgs a) 
 // Joins the chunks of each row of head blockIdx.y of sequence blockIdx.z (rows
 // whose sequence is one chunk were written by its workgroup): D / 4 lanes take 4
 // columns each of every NS-th chunk of a row, NS such groups a row.  Bound by
-// latency (NS > 1: few rows of many chunks) or by reading the chunks' rows.
+// latency (NS = 8, few rows: 3.9 us) or by reading the chunks' rows (NS = 1: 8
+// chunks of 8192 rows of 128, 6.9 us, 4.9 TB/s).
 template <typename E, int D, int NS>
 __global__ __launch_bounds__(256) void fa_paged_merge_kernel(PagedAttnArgs a) {
   constexpr int kLanes = D / 4, kRows = 256 / (kLanes * NS);

@@ -261,6 +261,9 @@ struct RotaryArgs {
 // cosines and sines of a token are shared by its heads: computed once per
 // workgroup into LDS, then read by one lane per unit.  Lanes keep their unit and
 // walk the (token, head) rows, so that the sweep has no division.
+// 4096 tokens of 40 heads of 128, bf16: 17.3 us, 4.9 TB/s, the rate of a large
+// copy (28 us with each column chunk loaded twice and an index divided a row);
+// 32 tokens: 3.5 us, launch and two load latencies.
 constexpr int kRotaryThreads = 256;
 
 __device__ __forceinline__ int64_t rotary_position(const void *positions, int pos64, int64_t i) {
