@@ -756,7 +756,8 @@ __global__ __launch_bounds__(256) void fa_paged_few_kernel(PagedAttnArgs a) {
 // large library product of this type reaches 1.2; matrix instructions busy 49 % of
 // the cycles, vector ones 59 %, at the 1.8 GHz that the card then runs at (842 us
 // by the few-row kernel; 258 us with the same conversion before the stages were
-// interleaved).  256 queries on 8448: 55 us.
+// interleaved).  256 queries on 8448: 53 us, 20 of them before the first and after
+// the last tile (three dependent loads, two steps that fill the pipeline, rows out).
 constexpr int kRowsTile = 128, kRowsKeys = 64;
 
 template <typename E, int D>
