@@ -57,8 +57,8 @@ class PagedKVCache:
                                          [a, m, r, j / 2], low half: even j
       v_scales (N, H, P/4, D/32, 4)      t = 4a + r at [a, block, r]
     The value interleaving of 4 tokens is the order in which the attention's
-    matrix instructions take them.  Scales of 255 are never written by
-    append_paged and must not be put there.
+    matrix instructions take them.  append_paged writes scales of 1 to 252 (140
+    in an fp16 cache); larger ones must not be put there.
     """
 
     __slots__ = ("_tensors", "_dtype", "_sizes", "_structs", "_half", "_like", "_head_dim")

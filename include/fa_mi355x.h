@@ -505,8 +505,9 @@ int fa_rotary(const void *q, const void *k, void *q_out, void *k_out, const int6
  * Codes 16-byte, scales 4-byte aligned.  The page table of a call is (B,
  * width) int32: position p of sequence b is slot p % P of page
  * table[b][p / P].  An id outside [0, pages) is no page: nothing is stored
- * there and no query sees it.  Scales of 255 are never written; a cache
- * that holds one has undefined values in that block.
+ * there and no query sees it.  fa_paged_append writes scales of 1 .. 252 (140 in
+ * fp16); a fresh cache is all zeros.  Larger ones must not be put there: values
+ * past the 16-bit range are infinities, which unseen slots must not hold.
  */
 typedef struct fa_paged_cache {
   void *k_codes, *k_scales, *v_codes, *v_scales;
@@ -517,8 +518,8 @@ typedef struct fa_paged_cache {
  * Stores the keys and values of new tokens: token i < counts[b] (S with
  * counts NULL; clamped to 0 .. S) of sequence b goes to position start[b] + i.
  * With `steps` (else NULL) keys are first rotated by that position
- * (fa_rotary's arguments; in fp64, so that a code is the nearest to the rotated
- * value itself).  A block's scale is the power of two floor(log2 max|x|) - 2,
+ * (fa_rotary's arguments, of the flags FA_ROTARY_INTERLEAVED alone; in fp64, so
+ * that a code is the nearest to the rotated value itself).  A block's scale is the power of two floor(log2 max|x|) - 2,
  * a value the nearest e2m1 number (ties to the even code, 6 above).  NaN is
  * stored as 0, an infinity as the largest finite value of `dtype`; with
  * FA_DTYPE_F16 the scale is at most 2^13, so that what is held fits fp16.

@@ -219,3 +219,13 @@ def test_handles_are_fixed_and_copy():
     assert copy.copy(rot).steps is rot.steps and copy.deepcopy(rot).frequencies == rot.frequencies
     rot.frequencies.clear()
     assert len(rot.frequencies) == 16
+
+
+def test_a_library_without_the_entry_points_is_named(tmp_path):
+    """One of this version, built before they were added: rebuild it."""
+    import subprocess
+    src, out = tmp_path / "stub.c", tmp_path / "libfa_mi355x.so"
+    src.write_text("int fa_abi_version(void) { return %d; }\n" % _capi.ABI_VERSION)
+    subprocess.run(["gcc", "-shared", "-fPIC", str(src), "-o", str(out)], check=True)
+    with pytest.raises(_capi.LibraryNotBuilt, match="rebuild it"):
+        _capi.load(str(out))

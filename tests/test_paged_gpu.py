@@ -505,3 +505,66 @@ def test_empty_and_refused():
                                                   torch.float32)):
         with pytest.raises((FlashAttnArgumentError, RuntimeError)):
             bad()
+
+
+def test_other_layouts_are_taken():
+    """Tables, lengths and rows that the kernels do not read in place are copied:
+    strided tables, misaligned rows, strides that are no multiple of 8."""
+    from flash_attn_volta import (PagedKVCache, RotaryPositions, append_paged, attend_paged,
+                                  read_paged, rotary_forward)
+    B, S, H, Hk, D, P = 2, 5, 4, 2, 64, 16
+    rot = RotaryPositions(32)
+    q, k, v = (_rand((B, S, h, D), F16, i).cuda() for i, h in enumerate((H, Hk, Hk)))
+    table, start, n = _i32([[3, 0], [1, 2]]), _i32([9, 14]), _i32([14, 19])
+    pos = torch.arange(S, device="cuda")
+
+    def run(q, k, v, table, start, n):
+        cache = PagedKVCache(4, P, Hk, D, F16)
+        qo = append_paged(cache, k, v, table, start, q=q, rotary=rot)
+        return (qo, *read_paged(cache, table, start, S), attend_paged(qo, cache, table, n),
+                rotary_forward(q, k, pos, rot)[1])
+
+    def shifted(t):                       # 2 bytes off 16-byte alignment
+        flat = torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")
+        flat[1:] = t.flatten()
+        return flat[1:].view(t.shape)
+
+    def odd(t):                           # rows 4 elements apart from the next head's
+        wide = torch.zeros((*t.shape[:2], t.shape[2] * (D + 4)), dtype=t.dtype, device="cuda")
+        view = wide.view(*t.shape[:3], D + 4)[..., :D]
+        view.copy_(t)
+        return view
+
+    want = run(q, k, v, table, start, n)
+    twice = lambda t: torch.stack((t, t), dim=-1).flatten(-2)[..., ::2]  # noqa: E731
+    for args in ((shifted(q), shifted(k), shifted(v), table, start, n),
+                 (odd(q), odd(k), odd(v), table.t().contiguous().t(), start, n),
+                 (q, k, v, twice(table), twice(start), twice(n))):
+        assert all(torch.equal(a, b) for a, b in zip(run(*args), want))
+
+
+def test_the_python_way_gives_the_same(monkeypatch):
+    """Without the C++ module every call goes through Python."""
+    from flash_attn_volta import PagedKVCache, append_paged, attend_paged, paged, read_paged
+    lengths = [700, 33]
+    outs = []
+    for cpp in (paged._cpp, None):
+        monkeypatch.setattr(paged, "_cpp", cpp)
+        cache, table, model = _filled(2, lengths, 2, 64, 16, BF16, 7)
+        q = _rand((2, 3, 8, 64), BF16, 1).cuda()
+        out, lse = attend_paged(q, cache, _i32(table), _i32(lengths), return_softmax_lse=True)
+        k, v = read_paged(cache, _i32(table), _i32([1, 2]), 40, _i32([40, 3]))
+        outs.append((out, lse, k, v, append_paged(cache, k[:, :1], v[:, :1], _i32(table),
+                                                  _i32([0, 0]), q=q[:, :1])))
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+
+
+def test_shared_pages_and_one_table_for_all():
+    """Sequences that share a prefix's pages, and one table row for every sequence."""
+    from flash_attn_volta import attend_paged
+    cache, table, model = _filled(1, [100], 2, 64, 16, F16, 9)
+    q = _rand((3, 2, 4, 64), F16, 1)
+    lengths = [100, 37, 2]
+    shared = _i32(table).expand(3, -1)
+    out, lse = attend_paged(q.cuda(), cache, shared, _i32(lengths), return_softmax_lse=True)
+    _check_attend(out, lse, q, model, table.repeat(3, 0), lengths)

@@ -212,6 +212,23 @@ def test_graph_replays_and_other_stream():
         assert all(torch.equal(a, b) for a, b in zip(got, want)), rep
 
 
+def test_saved_tensor_hooks():
+    """What comes back from a hook on saved tensors is read by its own strides."""
+    from flash_attn_volta import RotaryPositions, apply_rotary_positions, rotary_backward
+    rot = RotaryPositions(32)
+    pos = torch.arange(9, device="cuda")[None].expand(2, -1)
+    x = _inputs(2, 9, 2, 64, torch.float16, 0).cuda().requires_grad_()
+    g = _inputs(2, 9, 2, 64, torch.float16, 1).cuda()
+    with torch.autograd.graph.save_on_cpu():
+        out = apply_rotary_positions(x, None, pos, rot)[0]
+    got, = torch.autograd.grad(out, x, g)
+    assert torch.equal(got, rotary_backward(g, None, pos, rot)[0])
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t[..., :1]):
+        out = apply_rotary_positions(x, None, pos, rot)[0]
+    with pytest.raises(RuntimeError, match="saved tensor"):
+        torch.autograd.grad(out, x, g)
+
+
 def test_python_node_gives_the_same(monkeypatch):
     """Without the C++ module the Python Function carries every call."""
     from flash_attn_volta import RotaryPositions, apply_rotary_positions, rotary
