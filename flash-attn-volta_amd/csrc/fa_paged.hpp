@@ -656,11 +656,12 @@ __global__ __launch_bounds__(256) void fa_paged_few_kernel(PagedAttnArgs a) {
 #pragma unroll
       for (int i = 1; i < 8; ++i) top = fmaxf(top, s[i >> 2][nt][i & 3]);
       top *= a.c;
-      // a new maximum only where the old one is left behind by 2^8
+      // a new maximum only for rows whose old one is left behind by 2^8: no row's
+      // rounding depends on the other rows of its tile
       if (__any(top > mx[nt] + 8.0f)) {
         float t = fmaxf(top, __shfl_xor(top, 16, 64));
         t = fmaxf(t, xor32(t));
-        t = fmaxf(t, mx[nt]);
+        t = t > mx[nt] + 8.0f ? t : mx[nt];
         const float f = fast_exp2(mx[nt] - t);
         mx[nt] = t;
         l[nt] *= f;
@@ -847,8 +848,8 @@ __global__ __launch_bounds__(256, 2) void fa_paged_rows_kernel(PagedAttnArgs a) 
   auto v_frag = [&](int buf, int i) {   // of V instruction i: keys i / ND, tile i % ND
     return __builtin_bit_cast(vec8<E>, s_v[buf][2 * (i / ND) + hf][i % ND][n]);
   };
-  // masks tile `key`'s scores, and moves the running maximum where they leave the
-  // old one behind by 2^8
+  // masks tile `key`'s scores, and moves the running maximum of the rows where they
+  // leave the old one behind by 2^8 (of no other row: none depends on its neighbours)
   const int lim = min(last, end - 1);   // the last position that this lane's row sees here
   auto settle = [&](int key, int buf, floatx16 (&x)[2]) {
     if (key + kRowsKeys > all || key + kRowsKeys > end) {
@@ -869,7 +870,8 @@ __global__ __launch_bounds__(256, 2) void fa_paged_rows_kernel(PagedAttnArgs a) 
     for (int i = 1; i < 32; ++i) top = fmaxf(top, x[i >> 4][i & 15]);
     top *= a.c;
     if (__any(top > mx + 8.0f)) {
-      const float t = fmaxf(max_xor32(top), mx);
+      float t = max_xor32(top);
+      t = t > mx + 8.0f ? t : mx;
       const float f = fast_exp2(mx - t);
       mx = t;
       l *= f;
