@@ -223,7 +223,15 @@ AttnPlan attn_plan(int B, int Sq, int H, int Hk, int cus, int64_t capacity) {
   // (2 with two column tiles: 16 x 4 queries of 14 / 2 heads of 64 on up to 5000
   // tokens 8.9 us, 11.4 with 4), the many-row one 2.
   const int64_t resident = (int64_t)(p.nt == 1 ? 4 : 2) * cus / ((int64_t)Hk * p.row_tiles);
-  p.target = resident < 1 || capacity <= fa::kUnit ? 1 : (int)resident;   // (a unit is never split)
+  // Where a table holds few positions no sequence is split: the join costs more than
+  // the sweeps (us, split / not, 32 / 8 heads of 128: one query of 1, 8 and 32
+  // sequences on 512 tokens 8.9 / 6.3, 8.8 / 6.8, 11.3 / 6.9; on 1024 9.0 / 8.9, 9.1 /
+  // 9.4, 13.1 / 10.1; on 2048 9.0 / 14.6, 11.7 / 15.2, 19.8 / 16.2: the 32 have a
+  // workgroup for each compute unit unsplit; 256 on 512 22 / 17, on 1024 31 / 26, on
+  // 1500 31 / 36).
+  const bool every_cu = p.nt != 0 && (int64_t)B * Hk * p.row_tiles >= cus;
+  const int64_t enough = p.nt == 0 ? 1024 : (every_cu ? 2048 : 512);
+  p.target = resident < 1 || capacity <= enough ? 1 : (int)resident;
   p.slots = p.target > 1 ? std::max(p.target, (p.target + 1) / 2 + B) : B;   // fa::find_chunk
   // (no more than the units that the table holds)
   const int64_t units = (std::min(capacity, (int64_t)1 << 30) + fa::kUnit - 1) / fa::kUnit;

@@ -568,3 +568,53 @@ def test_shared_pages_and_one_table_for_all():
     shared = _i32(table).expand(3, -1)
     out, lse = attend_paged(q.cuda(), cache, shared, _i32(lengths), return_softmax_lse=True)
     _check_attend(out, lse, q, model, table.repeat(3, 0), lengths)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("Sq,H,Hk,D", [(1, 8, 2, 128), (5, 6, 2, 64), (3, 4, 4, 32), (40, 4, 1, 128),
+                                       (150, 8, 4, 32), (70, 16, 2, 64), (41, 14, 2, 128)])
+def test_attend_split_padded(dtype, Sq, H, Hk, D):
+    """Tables large enough that long sequences are split and joined, beside short,
+    empty and padded ones: counts, holes, early rows that see nothing."""
+    from flash_attn_volta import attend_paged
+    lengths, counts = [1500, 47, 3, 0, 130, 700], [Sq, 1, 0, Sq, Sq // 2, Sq]
+    cache, table, model = _filled(6, lengths, Hk, D, 16, dtype, 3, width=130)
+    table[0, 2], table[0, 60], table[4, 0], table[5, 43] = -1, -7, 2 ** 30, 6 * 130 + 3
+    q = _rand((6, Sq, H, D), dtype, 8)
+    for cnt in (counts, None):
+        out, lse = attend_paged(q.cuda(), cache, _i32(table), _i32(lengths),
+                                None if cnt is None else _i32(cnt), return_softmax_lse=True)
+        _check_attend(out, lse, q, model, table, lengths, cnt)
+
+
+@pytest.mark.parametrize("B,seed", [(63, 0), (64, 1), (65, 2), (130, 3)])
+def test_split_many_sequences(B, seed):
+    """More sequences than a wave counts at once, some of many chunks."""
+    from flash_attn_volta import attend_paged
+    rng = np.random.default_rng(seed)
+    lengths = [int(x) for x in rng.integers(0, 300, B)]
+    for i, n in ((0, 2600), (B // 2, 1900), (B - 1, 2570)):
+        lengths[i] = n
+    cache, table, model = _filled(B, lengths, 1, 32, 16, BF16, 4, width=165)
+    q = _rand((B, 1, 4, 32), BF16, 8)
+    out, lse = attend_paged(q.cuda(), cache, _i32(table), _i32(lengths), return_softmax_lse=True)
+    _check_attend(out, lse, q, model, table, lengths)
+
+
+@pytest.mark.parametrize("H,Hk,D,dtype", [(24, 12, 64, F16), (8, 8, 128, BF16), (4, 2, 32, BF16)])
+def test_prompt_in_pieces(H, Hk, D, dtype):
+    """A 1300-token prompt in pieces of odd sizes gives each row what it gets in one."""
+    from flash_attn_volta import attend_paged
+    L = 1300
+    cache, table, model = _filled(1, [L], Hk, D, 64, dtype, 2)
+    q = _rand((1, L, H, D), dtype, 6).cuda()
+    whole = attend_paged(q, cache, _i32(table), _i32([L]))
+    at = 0
+    # a probability and an output are rounded, half a step each, and twice: two calls
+    tol = 4 * 4 * torch.finfo(dtype).eps / 2
+    for n in (1, 2, 13, 64, 65, 300, 511, 344):
+        piece = attend_paged(q[:, at:at + n], cache, _i32(table), _i32([at + n]))
+        diff = (piece.float() - whole[:, at:at + n].float()).abs().max()
+        assert diff <= tol * whole[:, at:at + n].float().abs().max(), (at, n, float(diff))
+        at += n
+    assert at == L
