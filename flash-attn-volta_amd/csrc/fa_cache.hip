@@ -92,7 +92,7 @@ int check_rotary(const int64_t *steps, double factor, int rotary_dim, int D) {
   if (steps == nullptr) return FA_ERR_NULL_POINTER;
   if (!aligned(steps, 8)) return FA_ERR_ALIGNMENT;
   if (rotary_dim < 2 || rotary_dim > D || (rotary_dim & 1)) return FA_ERR_HEAD_DIM;
-  return isfinite(factor) ? FA_OK : FA_ERR_SCALE;
+  return isfinite((float)factor) ? FA_OK : FA_ERR_SCALE;   // (q is rotated in fp32)
 }
 
 int log2_up(int n) {

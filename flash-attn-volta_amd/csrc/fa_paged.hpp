@@ -153,7 +153,7 @@ __global__ __launch_bounds__(kAppendThreads) void fa_paged_append_kernel(AppendA
         });
     return;
   }
-  if (a.counts) nt = min(nt, a.counts[b] - i0);
+  if (a.counts) nt = min(nt, max(a.counts[b], 0) - i0);
   if (nt <= 0) return;
   CosSin<double> *cs = reinterpret_cast<CosSin<double> *>(smem);
   // 8 aligned positions are slots of one page
@@ -396,11 +396,14 @@ __device__ __forceinline__ bool find_chunk(const PagedAttnArgs &a, int want, boo
     out.keys = units * kUnit;
     return by_sequence || want < out.count;
   }
+  // Units of a chunk.  (2^23 are a whole sequence of any length; more of them, in a
+  // batch of over 2^31 keys, would leave the range of positions.)
+  auto share = [&](int total, int chunks) {
+    return min(max(1, (total - 1) / chunks + 1), 1 << 23);
+  };
   // Short last chunks can go over the target: then as many fewer whole ones as there
   // are sequences, half the target at least.
-  auto fewer = [&](int total) {
-    return max(1, (total - 1) / max(a.target - a.B, (a.target + 1) / 2) + 1);
-  };
+  auto fewer = [&](int total) { return share(total, max(a.target - a.B, (a.target + 1) / 2)); };
   int length = 0, held = 0;
   auto load = [&](int b) {              // units of sequence b, this lane's
     length = b < a.B ? a.lengths[b] : 0;
@@ -428,7 +431,7 @@ __device__ __forceinline__ bool find_chunk(const PagedAttnArgs &a, int want, boo
   auto last = [](int x) { return __builtin_amdgcn_readlane(x, 63); };
   if (a.B <= 64) {
     const int u = load(lane), total = last(wave_prefix(u));
-    int units = max(1, (total + a.target - 1) / a.target);
+    int units = share(total, a.target);
     int n = lane < a.B ? parts(u, units) : 0, upto = prefix(n);
     if ((last(upto) & 0xFFFF) > a.target) {
       units = fewer(total);
@@ -446,7 +449,7 @@ __device__ __forceinline__ bool find_chunk(const PagedAttnArgs &a, int want, boo
     return last(wave_prefix(x));
   };
   const int total = sum([](int u) { return u; });
-  int units = max(1, (total + a.target - 1) / a.target);
+  int units = share(total, a.target);
   if (sum([&](int u) { return parts(u, units); }) > a.target) units = fewer(total);
   int before = 0, before_split = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {

@@ -140,7 +140,14 @@ class RotaryPositions:
                  lambda: f"rotary_dim must be an even number from 2 to 256, got {rotary_dim!r}")
         _require(isinstance(base, (int, float)) and math.isfinite(base) and base > 0,
                  lambda: f"base must be a positive number, got {base!r}")
-        self._frequencies, factor = _scaled_frequencies(rotary_dim, float(base), scaling)
+        try:
+            self._frequencies, factor = _scaled_frequencies(rotary_dim, float(base), scaling)
+        except OverflowError:
+            self._frequencies, factor = [math.inf], 1.0
+        _require(all(map(math.isfinite, self._frequencies)),
+                 lambda: f"base {base!r} and this scaling give frequencies that are not finite")
+        _require(factor <= torch.finfo(torch.float32).max,
+                 lambda: f"attention_factor {factor!r} is over fp32's largest number")
         steps = torch.tensor([_step(f) for f in self._frequencies], dtype=torch.int64, device=device)
         # (fixed: the kernels read rotary_dim / 2 steps)
         self._args = (steps, factor, rotary_dim, _capi.FA_ROTARY_INTERLEAVED if interleaved else 0)

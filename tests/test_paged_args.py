@@ -229,3 +229,15 @@ def test_a_library_without_the_entry_points_is_named(tmp_path):
     subprocess.run(["gcc", "-shared", "-fPIC", str(src), "-o", str(out)], check=True)
     with pytest.raises(_capi.LibraryNotBuilt, match="rebuild it"):
         _capi.load(str(out))
+
+
+def test_numbers_out_of_range(lib):
+    """Factors and frequencies that leave fp32's or Python's range are refused."""
+    from flash_attn_volta import RotaryPositions
+    from flash_attn_volta.forward import FlashAttnArgumentError
+    assert _rotary(lib, factor=1e39) == _capi.FA_ERR_SCALE
+    for kw in (dict(base=5e-324), dict(scaling={"type": "linear", "factor": 5e-324}),
+               dict(base=1e300, scaling={"type": "ntk", "factor": 1e300}),
+               dict(scaling={"type": "factors", "factors": [1.0] * 32, "attention_factor": 1e39})):
+        with pytest.raises(FlashAttnArgumentError):
+            RotaryPositions(64, device="cpu", **kw)

@@ -618,3 +618,54 @@ def test_prompt_in_pieces(H, Hk, D, dtype):
         assert diff <= tol * whole[:, at:at + n].float().abs().max(), (at, n, float(diff))
         at += n
     assert at == L
+
+
+@pytest.mark.parametrize("Sq,H,L", [(5, 2, 400), (8, 8, 400), (300, 2, 900), (40, 2, 2100)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_a_row_does_not_depend_on_its_neighbours(dtype, Sq, H, L):
+    """Bit for bit: queries with scores far larger, in rows of the same tiles, move
+    no other row's running maximum."""
+    from flash_attn_volta import attend_paged
+    cache, table, _ = _filled(1, [L], 1, 64, 16, dtype, 5)
+    q = _rand((1, Sq, H, 64), dtype, 7)
+    loud = q.clone()
+    loud[:, 1::2] *= 40
+    a, b = (attend_paged(x.cuda(), cache, _i32(table), _i32([L])) for x in (q, loud))
+    assert torch.equal(a[:, ::2], b[:, ::2])
+    assert not torch.equal(a[:, 1::2], b[:, 1::2])
+
+
+def test_counts_below_zero_are_none():
+    from flash_attn_volta import PagedKVCache, append_paged, attend_paged, read_paged
+    low = -2 ** 31
+    cache, table = PagedKVCache(4, 16, 2, 32, BF16), _i32([[0, 1]])
+    k, v, q = (_rand((1, 24, 2, 32), BF16, i).cuda() for i in range(3))
+    for n in (low, low + 5, -1):
+        append_paged(cache, k, v, table, _i32([3]), _i32([n]))
+        assert not any(getattr(cache, t).any() for t in ("k_codes", "k_scales", "v_codes", "v_scales"))
+    append_paged(cache, k, v, table, _i32([0]))
+    for n in (low, -1):
+        assert not any(t.any() for t in read_paged(cache, table, _i32([0]), 24, _i32([n])))
+        out, lse = attend_paged(q, cache, table, _i32([24]), _i32([n]), return_softmax_lse=True)
+        assert not out.any() and torch.isinf(lse).all()
+        assert not attend_paged(q, cache, table, _i32([n])).any()
+
+
+def test_a_batch_of_over_2_31_keys():
+    """Sequences that share one page hold 2^30 keys each, of which no query is asked;
+    the one beside them keeps its result.  (Over 1024 heads: no sequence is split.)"""
+    from flash_attn_volta import PagedKVCache, append_paged, attend_paged
+    P, H, L = 4096, 1025, 100
+    cache = PagedKVCache(1, P, H, 32, BF16)
+    k, v, q = (_rand((1, n, H, 32), BF16, i).cuda() for i, n in enumerate((L, L, 1)))
+    one = torch.zeros((1, 2 ** 30 // P), dtype=torch.int32, device="cuda")
+    append_paged(cache, k, v, one, _i32([0]))
+    alone = attend_paged(q, cache, one, _i32([L]))
+    assert alone.any()
+    for at in range(3):
+        lengths, counts = [2 ** 30] * 3, [0] * 3
+        lengths[at], counts[at] = L, 1
+        out = attend_paged(q.expand(3, -1, -1, -1), cache, one.expand(3, -1), _i32(lengths),
+                           _i32(counts))
+        assert torch.equal(out[at], alone[0])
+        assert not out[[i for i in range(3) if i != at]].any()
