@@ -561,7 +561,9 @@ size_t fa_paged_attn_workspace_bytes(int B, int Sq, int H, int Hk, int D);
  * every query behind counts[b], gets o = 0 and lse = +inf.  Scores are fp32; keys
  * and values enter the products as the exact 16-bit values of their codes (fp16:
  * rounded below 2^-24).  The lengths are read on the device, which shares all
- * sequences' keys out evenly whatever they are.
+ * sequences' keys out evenly whatever they are (in tables for more than a few
+ * hundred positions; in smaller ones a workgroup takes a sequence).  A row's bits
+ * depend on the lengths of the batch, not on the other rows.
  * q (B, Sq, H, D); o (B, Sq, H, D) contiguous; lse (B, H, Sq) fp32 or NULL; query
  * head h reads head h / (H / heads).  At most 2^20 rows a head of the cache (Sq
  * H / heads) and 2^30 positions a sequence (width * P), else FA_ERR_TOO_LARGE.

@@ -669,3 +669,29 @@ def test_a_batch_of_over_2_31_keys():
                            _i32(counts))
         assert torch.equal(out[at], alone[0])
         assert not out[[i for i in range(3) if i != at]].any()
+
+
+def test_calls_inside_a_compiled_function():
+    """Traced functions call them between the pieces of their graphs."""
+    from flash_attn_volta import (PagedKVCache, RotaryPositions, append_paged,
+                                  apply_rotary_positions, attend_paged, read_paged)
+    rotary, pos = RotaryPositions(64), torch.arange(5, device="cuda")[None]
+    q, k = (_rand((2, 5, h, 64), F16, h).cuda().requires_grad_() for h in (8, 2))
+    table, start = _i32(np.arange(8).reshape(2, 4)), _i32([0, 3])
+
+    def train(q, k):
+        a, b = apply_rotary_positions(q * 2, k, pos, rotary)
+        return (a * b.repeat_interleave(4, 2)).float().sum()
+
+    def serve(q, k, cache):
+        rotated = append_paged(cache, k, k + 1, table, start, q=q, rotary=rotary)
+        out, lse = attend_paged(rotated * 1, cache, table, start + 5, return_softmax_lse=True)
+        return (out * 1, lse, *read_paged(cache, table, start, 5))
+
+    grads, results = [], []
+    for wrap in (lambda f: f, lambda f: torch.compile(f, backend="eager")):
+        grads.append(torch.autograd.grad(wrap(train)(q, k), (q, k)))
+        with torch.no_grad():
+            results.append(wrap(serve)(q, k, PagedKVCache(8, 16, 2, 64, F16)))
+    for a, b in (*zip(*grads), *zip(*results)):
+        assert torch.equal(a, b)
