@@ -386,6 +386,15 @@ __device__ __forceinline__ bool find_chunk(const PagedAttnArgs &a, int want, boo
     q += (q + 1) * units <= x ? 1 : 0;
     return max(1, q);
   };
+  if (a.target == 1) {                  // nothing is split: a slot is a sequence
+    out.b = want;
+    out.index = out.part = 0;
+    out.count = 1;
+    out.length = a.lengths[want];
+    out.held = held_keys(a, out.length);
+    out.keys = 1 << 30;
+    return true;
+  }
   if (a.B == 1) {                       // one user's tokens: scalar work alone
     out.b = out.part = 0;
     out.length = a.lengths[0];
@@ -440,11 +449,23 @@ __device__ __forceinline__ bool find_chunk(const PagedAttnArgs &a, int want, boo
     }
     return find(upto, n, 0, 0, 0, units);
   }
+  // 4 groups of 64 sequences at a time, their loads in flight together
+  constexpr int kGroups = 4;
+  int group[kGroups];
+  auto load_groups = [&](int b0) {
+#pragma unroll
+    for (int j = 0; j < kGroups; ++j) {
+      const int b = b0 + 64 * j + lane;
+      group[j] = b < a.B ? a.lengths[b] : 0;
+    }
+  };
   auto sum = [&](auto &&f) {            // over all sequences
     int x = 0;
-    for (int b0 = 0; b0 < a.B; b0 += 64) {
-      const int u = load(b0 + lane);
-      x += b0 + lane < a.B ? f(u) : 0;
+    for (int b0 = 0; b0 < a.B; b0 += 64 * kGroups) {
+      load_groups(b0);
+#pragma unroll
+      for (int j = 0; j < kGroups; ++j)
+        x += b0 + 64 * j + lane < a.B ? f(units_of(held_keys(a, group[j]))) : 0;
     }
     return last(wave_prefix(x));
   };
@@ -452,12 +473,18 @@ __device__ __forceinline__ bool find_chunk(const PagedAttnArgs &a, int want, boo
   int units = share(total, a.target);
   if (sum([&](int u) { return parts(u, units); }) > a.target) units = fewer(total);
   int before = 0, before_split = 0;
-  for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const int u = load(b0 + lane), n = b0 + lane < a.B ? parts(u, units) : 0;
-    const int upto = prefix(n);
-    if (find(upto, n, b0, before, before_split, units)) return true;
-    before += last(upto) & 0xFFFF;
-    before_split += last(upto) >> 16;
+  for (int b0 = 0; b0 < a.B; b0 += 64 * kGroups) {
+    load_groups(b0);
+#pragma unroll
+    for (int j = 0; j < kGroups; ++j) {
+      const int at = b0 + 64 * j;
+      length = group[j];
+      held = held_keys(a, length);
+      const int n = at + lane < a.B ? parts(units_of(held), units) : 0, upto = prefix(n);
+      if (find(upto, n, at, before, before_split, units)) return true;
+      before += last(upto) & 0xFFFF;
+      before_split += last(upto) >> 16;
+    }
   }
   return false;
 }

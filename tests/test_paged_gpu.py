@@ -695,3 +695,41 @@ def test_calls_inside_a_compiled_function():
             results.append(wrap(serve)(q, k, PagedKVCache(8, 16, 2, 64, F16)))
     for a, b in (*zip(*grads), *zip(*results)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("B,Sq,Hk", [(255, 1, 1), (256, 4, 2), (257, 1, 1), (515, 1, 1), (300, 140, 1)])
+def test_split_hundreds_of_sequences(B, Sq, Hk):
+    """As test_split_many_sequences, with more sequences and rows; and the same batch in
+    a table that is not split."""
+    from flash_attn_volta import attend_paged
+    rng = np.random.default_rng(B)
+    lengths = [int(x) for x in rng.integers(0, 150, B)]
+    for i, n in ((1, 2100), (B // 2, 0), (B - 1, 2111)):
+        lengths[i] = n
+    cache, table, model = _filled(B, lengths, Hk, 32, 16, F16, 4, width=132)
+    q = _rand((B, Sq, Hk, 32), F16, 8)
+    out, lse = attend_paged(q.cuda(), cache, _i32(table), _i32(lengths), return_softmax_lse=True)
+    _check_attend(out, lse, q, model, table, lengths)
+    short = [min(n, 500) for n in lengths]
+    out, lse = attend_paged(q.cuda(), cache, _i32(table[:, :32]), _i32(short),
+                            return_softmax_lse=True)
+    _check_attend(out, lse, q, model, table[:, :32], short)
+
+
+def test_a_batch_of_over_2_32_keys_that_may_be_split():
+    """As test_a_batch_of_over_2_31_keys, with chunks in reach: 512 heads, two a round."""
+    from flash_attn_volta import PagedKVCache, append_paged, attend_paged
+    P, H, L, B = 4096, 512, 100, 6
+    cache = PagedKVCache(1, P, H, 32, F16)
+    k, v, q = (_rand((1, n, H, 32), F16, i).cuda() for i, n in enumerate((L, L, 1)))
+    one = torch.zeros((1, 2 ** 30 // P), dtype=torch.int32, device="cuda")
+    append_paged(cache, k, v, one, _i32([0]))
+    alone = attend_paged(q, cache, one[:, :1], _i32([L]))
+    assert alone.any()
+    for at in (0, 3, 5):
+        lengths, counts = [2 ** 30] * B, [0] * B
+        lengths[at], counts[at] = L, 1
+        out = attend_paged(q.expand(B, -1, -1, -1), cache, one.expand(B, -1), _i32(lengths),
+                           _i32(counts))
+        assert torch.equal(out[at], alone[0])
+        assert not out[[i for i in range(B) if i != at]].any()
