@@ -201,8 +201,10 @@ struct AttnPlan {
   size_t o_bytes(int Hk, int D) const {
     return target > 1 ? (size_t)(target + 1) * Hk * rows * D * sizeof(float) : 0;
   }
-  size_t bytes(int Hk, int D) const {
-    return target > 1 ? o_bytes(Hk, D) + (size_t)(target + 1) * Hk * rows * 2 * sizeof(float) : 0;
+  size_t bytes(int B, int Hk, int D) const {
+    return target > 1 ? o_bytes(Hk, D) + (size_t)(target + 1) * Hk * rows * 2 * sizeof(float) +
+                            (B > 1 ? (size_t)B * 2 * sizeof(int) : 0)
+                      : 0;
   }
 };
 
@@ -265,10 +267,12 @@ int launch_attn(const fa::PagedAttnArgs &a, const AttnPlan &p, hipStream_t st) {
     const int64_t each = kGroups / ns;
     return dim3((unsigned)((p.rows + each - 1) / each), (unsigned)a.cache.Hk, (unsigned)a.B);
   };
-  if (p.rows * a.cache.Hk * a.B >= (int64_t)4 * kGroups * stream_cus(st))
-    fa::fa_paged_merge_kernel<E, D, 1><<<blocks(1), 256, 0, st>>>(a);
-  else
-    fa::fa_paged_merge_kernel<E, D, 8><<<blocks(8), 256, 0, st>>>(a);
+  const bool many = p.rows * a.cache.Hk * a.B >= (int64_t)4 * kGroups * stream_cus(st);
+  const auto merge = a.B == 1 ? (many ? fa::fa_paged_merge_kernel<E, D, 1, true>
+                                      : fa::fa_paged_merge_kernel<E, D, 8, true>)
+                              : (many ? fa::fa_paged_merge_kernel<E, D, 1, false>
+                                      : fa::fa_paged_merge_kernel<E, D, 8, false>);
+  merge<<<blocks(many ? 1 : 8), 256, 0, st>>>(a);
   return launch_status();
 }
 
@@ -411,7 +415,7 @@ int fa_paged_read(const fa_paged_cache *cache, const int32_t *table, int64_t tab
 
 size_t fa_paged_attn_workspace_bytes(int B, int Sq, int H, int Hk, int D) {
   if (check_attn_sizes(B, Sq, H, Hk, D, FA_DTYPE_F16) != FA_OK) return 0;
-  return attn_plan(B, Sq, H, Hk, stream_cus(nullptr), INT64_MAX).bytes(Hk, D);
+  return attn_plan(B, Sq, H, Hk, stream_cus(nullptr), INT64_MAX).bytes(B, Hk, D);
 }
 
 int fa_paged_attn(const void *q, const fa_paged_cache *cache, const int32_t *table,
@@ -431,8 +435,8 @@ int fa_paged_attn(const void *q, const fa_paged_cache *cache, const int32_t *tab
   const int cus = stream_cus(st);
   const AttnPlan most = attn_plan(B, Sq, H, Hk, cus, INT64_MAX);
   if ((int64_t)most.slots * Hk > kMaxThreads / 256) return FA_ERR_TOO_LARGE;
-  if (most.bytes(Hk, D) > 0) {
-    if (workspace == nullptr || workspace_bytes < most.bytes(Hk, D)) return FA_ERR_WORKSPACE;
+  if (most.bytes(B, Hk, D) > 0) {
+    if (workspace == nullptr || workspace_bytes < most.bytes(B, Hk, D)) return FA_ERR_WORKSPACE;
     if (!aligned(workspace, 16)) return FA_ERR_ALIGNMENT;
   }
   const AttnPlan p = attn_plan(B, Sq, H, Hk, cus, (int64_t)cache->width * cache->page_size);

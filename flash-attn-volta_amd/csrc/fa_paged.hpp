@@ -326,11 +326,23 @@ struct PagedAttnArgs {
   const int32_t *lengths, *counts;      // counts: NULL = Sq everywhere
   float *part_o;                        // (target + 1, Hk, rows, D) unnormalised
   float *part_ml;                       // (target + 1, Hk, rows, 2): maximum (log2), sum
+                                        // then, with B > 1, (B, 2) int: Chunk::count, part
   int B, Sq, H, G;
   int target;                           // chunks aimed at
   float c;                              // |sm_scale| log2 e
   uint32_t flip;                        // sign bits xor-ed into q (negative scale)
 };
+
+// A value that the kernel does not write, at an address that is the same in every lane.
+__device__ __forceinline__ int scalar_load(const int32_t *p) {
+  return *reinterpret_cast<const __attribute__((address_space(4))) int32_t *>(
+      reinterpret_cast<uintptr_t>(p));
+}
+
+// Has these kernel arguments in registers at this point: they are loaded together,
+// where the compiler would load each before its first use and wait for it there.
+template <typename T> __device__ __forceinline__ void have_one(T x) { asm volatile("" : : "s"(x)); }
+template <typename... T> __device__ __forceinline__ void have(T... x) { (have_one(x), ...); }
 
 // Queries of a packed tile: row n of (b, hk) is query n / G of head hk G + n % G.
 // Keys a row sees: positions <= lengths - counts + query.
@@ -364,6 +376,28 @@ __device__ __forceinline__ int wave_prefix(int x) {
   return dpp_add<0x143, 0xC>(x);
 }
 
+__device__ __forceinline__ int units_of(int held) { return (held + kUnit - 1) / kUnit; }
+
+// ceil(u / units), 1 at least, u and units up to 2^23: an fp32 quotient, off by
+// one at most.
+__device__ __forceinline__ int parts(int u, int units) {
+  const int x = u + units - 1;
+  int q = (int)((float)x * __builtin_amdgcn_rcpf((float)units));
+  q -= q * units > x ? 1 : 0;
+  q += (q + 1) * units <= x ? 1 : 0;
+  return max(1, q);
+}
+
+// The chunks of a batch of one sequence (one user's tokens: scalar work alone).
+__device__ __forceinline__ void one_sequence(const PagedAttnArgs &a, Chunk &out) {
+  out.b = out.part = 0;
+  out.length = scalar_load(a.lengths);
+  out.held = held_keys(a, out.length);
+  const int u = units_of(out.held), units = parts(u, a.target);
+  out.count = parts(u, units);
+  out.keys = units * kUnit;
+}
+
 // Splits all sequences' keys evenly: chunks of the same whole number of units
 // (the last of a sequence shorter), `target` of them at most where that can be,
 // whatever the lengths.  The host knows no lengths; every wave counts them for
@@ -371,39 +405,25 @@ __device__ __forceinline__ int wave_prefix(int x) {
 // a chunk too, which writes its zeros.  max(target, (target + 1) / 2 + B) slots
 // cover every chunk, B with a target of 1 (then no sequence is split); those of
 // sequences that are split are target + 1 at most (n > 1 chunks are under twice
-// their units' share).  With `by_sequence` the argument is a sequence and its
-// chunks are returned.
-__device__ __forceinline__ bool find_chunk(const PagedAttnArgs &a, int want, bool by_sequence,
-                                           Chunk &out) {
+// their units' share).  The first chunk of each of several sequences leaves its count for
+// the join, which would be longer over finding it than over joining (us with a join that
+// counts: 32 sequences on up to 3001 tokens 19.8, now 19.3, 128 on 4000 109, now 105;
+// a single sequence, which needs no counting, would lose 0.3).
+__device__ __forceinline__ bool find_chunk(const PagedAttnArgs &a, int want, Chunk &out) {
   const int lane = threadIdx.x & 63;
-  auto units_of = [&](int held) { return (held + kUnit - 1) / kUnit; };
-  // ceil(u / units), 1 at least, u and units up to 2^23: an fp32 quotient, off by
-  // one at most
-  auto parts = [&](int u, int units) {
-    const int x = u + units - 1;
-    int q = (int)((float)x * __builtin_amdgcn_rcpf((float)units));
-    q -= q * units > x ? 1 : 0;
-    q += (q + 1) * units <= x ? 1 : 0;
-    return max(1, q);
-  };
   if (a.target == 1) {                  // nothing is split: a slot is a sequence
     out.b = want;
     out.index = out.part = 0;
     out.count = 1;
-    out.length = a.lengths[want];
+    out.length = scalar_load(a.lengths + want);
     out.held = held_keys(a, out.length);
     out.keys = 1 << 30;
     return true;
   }
-  if (a.B == 1) {                       // one user's tokens: scalar work alone
-    out.b = out.part = 0;
-    out.length = a.lengths[0];
-    out.held = held_keys(a, out.length);
-    const int u = units_of(out.held), units = parts(u, a.target);
-    out.count = parts(u, units);
+  if (a.B == 1) {
+    one_sequence(a, out);
     out.index = want;
-    out.keys = units * kUnit;
-    return by_sequence || want < out.count;
+    return want < out.count;
   }
   // Units of a chunk.  (2^23 are a whole sequence of any length; more of them, in a
   // batch of over 2^31 keys, would leave the range of positions.)
@@ -424,7 +444,7 @@ __device__ __forceinline__ bool find_chunk(const PagedAttnArgs &a, int want, boo
   auto prefix = [&](int n) { return wave_prefix(n | (n > 1 ? n << 16 : 0)); };
   auto find = [&](int upto, int n, int b0, int before, int before_split, int units) {
     const int first = before + (upto & 0xFFFF) - n;
-    const bool mine = by_sequence ? b0 + lane == want : (want >= first && want < first + n);
+    const bool mine = want >= first && want < first + n;
     const uint64_t hit = __ballot(mine);
     if (!hit) return false;
     const int src = __builtin_ctzll(hit);
@@ -489,6 +509,19 @@ __device__ __forceinline__ bool find_chunk(const PagedAttnArgs &a, int want, boo
   return false;
 }
 
+__device__ __forceinline__ int *chunk_counts(const PagedAttnArgs &a) {
+  return reinterpret_cast<int *>(a.part_ml + (int64_t)(a.target + 1) * a.cache.Hk * (a.Sq * a.G) * 2);
+}
+
+// (by the first workgroup of a sequence, where any may be split)
+__device__ __forceinline__ void leave_count(const PagedAttnArgs &a, const Chunk &ch, int hk) {
+  if (a.B > 1 && a.target > 1 && ch.index == 0 && (hk | blockIdx.y | threadIdx.x) == 0) {
+    int *to = chunk_counts(a) + 2 * ch.b;
+    to[0] = ch.count;
+    to[1] = ch.part;
+  }
+}
+
 template <int D> struct KRaw { u32x4 w; };
 template <> struct KRaw<64> { u32x2 w; };
 template <> struct KRaw<32> { uint32_t w; };
@@ -508,11 +541,8 @@ template <int D> struct Tile16 {
 // that is none (page 0 is read instead, its keys masked).
 __device__ __forceinline__ int64_t tile_row(const PagedCache &c, int b, int hk, int key, int end,
                                             bool &hole) {
-  // (the id is loaded whether it is needed or not: no branch in the sweeps; as a
-  // constant: a scalar load)
-  typedef const __attribute__((address_space(4))) int32_t *Constants;
-  const int page = reinterpret_cast<Constants>(
-      reinterpret_cast<uintptr_t>(c.table))[b * c.table_stride + min(key >> c.page_shift, c.width - 1)];
+  // (the id is loaded whether it is needed or not: no branch in the sweeps)
+  const int page = scalar_load(c.table + b * c.table_stride + min(key >> c.page_shift, c.width - 1));
   hole = key >= end || (unsigned)page >= (unsigned)c.n_pages;
   return paged_row(c, hole ? 0 : page, hk, key & ((1 << c.page_shift) - 1));
 }
@@ -599,11 +629,13 @@ __global__ __launch_bounds__(256) void fa_paged_few_kernel(PagedAttnArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int Hk = a.cache.Hk, hk = blockIdx.x % Hk, slot = blockIdx.x / Hk;
+  have(a.cache.k_codes, a.cache.k_scales, a.cache.v_codes, a.cache.v_scales, a.cache.table,
+       a.cache.table_stride, a.cache.n_pages, a.cache.width);
   Chunk ch;
-  if (!find_chunk(a, slot, false, ch)) return;
+  if (!find_chunk(a, slot, ch)) return;
   const int b = ch.b, rows = a.Sq * a.G, row0 = blockIdx.y * (16 * NT);
   const int held = ch.held;
-  const int count = a.counts ? min(max(a.counts[b], 0), a.Sq) : a.Sq;
+  const int count = a.counts ? min(max(scalar_load(a.counts + b), 0), a.Sq) : a.Sq;
   const int base = ch.length - count;             // position of query 0
 
   // Q as B operands: column n = row0 + 16 nt + m, d = (D/4) g + 8 t + 0..7
@@ -781,6 +813,7 @@ __global__ __launch_bounds__(256) void fa_paged_few_kernel(PagedAttnArgs a) {
   else
     leave(std::integral_constant<int, 1>{});
   if (tid % lanes != 0) return;
+  leave_count(a, ch, hk);
   if (!whole) {
     a.part_ml[part * 2] = top;
     a.part_ml[part * 2 + 1] = real ? sum : 0.0f;
@@ -824,10 +857,10 @@ __global__ __launch_bounds__(256, 2) void fa_paged_rows_kernel(PagedAttnArgs a) 
   const int n = lane & 31, hf = lane >> 5;             // as an owner of row n
   const int Hk = a.cache.Hk, hk = blockIdx.x % Hk, slot = blockIdx.x / Hk;
   Chunk ch;
-  if (!find_chunk(a, slot, false, ch)) return;
+  if (!find_chunk(a, slot, ch)) return;
   const int b = ch.b, rows = a.Sq * a.G;
   const int row0 = (gridDim.y - 1 - blockIdx.y) * kRowsTile;   // the longest sweeps first
-  const int count = a.counts ? min(max(a.counts[b], 0), a.Sq) : a.Sq;
+  const int count = a.counts ? min(max(scalar_load(a.counts + b), 0), a.Sq) : a.Sq;
   const int base = ch.length - count;
 
   const int row = row0 + 32 * w + n, qi = row / a.G;
@@ -996,6 +1029,7 @@ __global__ __launch_bounds__(256, 2) void fa_paged_rows_kernel(PagedAttnArgs a) 
     }
   }
 
+  leave_count(a, ch, hk);
   // Rows leave through LDS: a lane holds 8 pieces of 2 ND columns of one row, and
   // stores of those would each touch as many lines as lanes (7000 cycles of a
   // workgroup, a third of a short sweep).  Piece mm of row n is kept at mm ^ n % 16.
@@ -1052,18 +1086,28 @@ __global__ __launch_bounds__(256, 2) void fa_paged_rows_kernel(PagedAttnArgs a) 
 // columns each of every NS-th chunk of a row, NS such groups a row.  Bound by
 // latency (NS = 8, few rows: 3.9 us) or by reading the chunks' rows (NS = 1: 8
 // chunks of 8192 rows of 128, 6.9 us, 4.9 TB/s).
-template <typename E, int D, int NS>
+template <typename E, int D, int NS, bool ONE>
 __global__ __launch_bounds__(256) void fa_paged_merge_kernel(PagedAttnArgs a) {
   constexpr int kLanes = D / 4, kRows = 256 / (kLanes * NS);
   const int hk = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
+  have(a.lengths, a.part_o, a.part_ml, a.o, a.lse, a.cache.width, a.cache.page_shift, a.cache.Hk,
+       a.Sq, a.G, a.H, a.target);
   const int rows = a.Sq * a.G, Hk = a.cache.Hk;
-  Chunk ch;
-  find_chunk(a, b, true, ch);
-  if (ch.count == 1) return;
+  int count, first = 0;
+  if constexpr (ONE) {
+    Chunk ch;
+    one_sequence(a, ch);
+    count = ch.count;
+  } else {
+    const int *left = chunk_counts(a) + 2 * b;
+    count = scalar_load(left);
+    first = scalar_load(left + 1);
+  }
+  if (count == 1) return;
   const int d4 = tid % kLanes, group = tid / kLanes, sub = group % NS;
   const int mine = group / NS, row = blockIdx.x * kRows + mine;
   const bool real = row < rows;
-  const int chunks = real ? ch.count : 0;
+  const int chunks = real ? count : 0;
   float top = kLowest, sum = 0.0f;
   floatx4 acc = {0, 0, 0, 0};
   for (int k0 = sub; k0 < chunks; k0 += 4 * NS) {        // 4 chunks' loads in flight
@@ -1071,8 +1115,8 @@ __global__ __launch_bounds__(256) void fa_paged_merge_kernel(PagedAttnArgs a) {
     floatx4 x[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int k = min(k0 + j * NS, ch.count - 1);
-      const int64_t p = ((int64_t)(ch.part + k) * Hk + hk) * rows + row;
+      const int k = min(k0 + j * NS, count - 1);
+      const int64_t p = ((int64_t)(first + k) * Hk + hk) * rows + row;
       const floatx2 ml = *reinterpret_cast<const floatx2 *>(a.part_ml + p * 2);
       mk[j] = ml[0];
       lk[j] = ml[1];
@@ -1080,7 +1124,7 @@ __global__ __launch_bounds__(256) void fa_paged_merge_kernel(PagedAttnArgs a) {
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      if (k0 + j * NS >= ch.count) break;
+      if (k0 + j * NS >= count) break;
       const float t = fmaxf(top, mk[j]), f0 = fast_exp2(top - t), f1 = fast_exp2(mk[j] - t);
       top = t;
       sum = sum * f0 + lk[j] * f1;
