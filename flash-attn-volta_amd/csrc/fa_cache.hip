@@ -208,7 +208,7 @@ struct AttnPlan {
   }
 };
 
-AttnPlan attn_plan(int B, int Sq, int H, int Hk, int cus, int64_t capacity) {
+AttnPlan attn_plan(int B, int Sq, int H, int Hk, int D, int cus, int64_t capacity) {
   AttnPlan p;
   p.rows = (int64_t)Sq * (H / Hk);
   // The many-row kernel pays from 65 rows on, from 257 where a call has at most
@@ -226,13 +226,21 @@ AttnPlan attn_plan(int B, int Sq, int H, int Hk, int cus, int64_t capacity) {
   // tokens 8.9 us, 11.4 with 4), the many-row one 2.
   const int64_t resident = (int64_t)(p.nt == 1 ? 4 : 2) * cus / ((int64_t)Hk * p.row_tiles);
   // Where a table holds few positions no sequence is split: the join costs more than
-  // the sweeps (us, split / not, 32 / 8 heads of 128: one query of 1, 8 and 32
-  // sequences on 512 tokens 8.9 / 6.3, 8.8 / 6.8, 11.3 / 6.9; on 1024 9.0 / 8.9, 9.1 /
-  // 9.4, 13.1 / 10.1; on 2048 9.0 / 14.6, 11.7 / 15.2, 19.8 / 16.2: the 32 have a
-  // workgroup for each compute unit unsplit; 256 on 512 22 / 17, on 1024 31 / 26, on
-  // 1500 31 / 36).
+  // the sweeps, whose steps take longer with wider rows and two tiles (us, split /
+  // whole: one query of 32 / 8 heads of 128 on 1024 tokens 9.3 / 9.0, on 1280 9.5 /
+  // 10.5; of 14 / 2 of 64 on 1280 9.3 / 8.2, on 1536 9.3 / 9.2, on 2048 9.4 / 11.3; 8
+  // queries of 32 / 8 of 128 on 512 9.5 / 8.9, on 768 9.6 / 10.9; 16 of 14 / 2 of 64 on
+  // 1024 9.7 / 8.9).  With a workgroup for each compute unit anyway: 32 x 1 of 32 / 8 of
+  // 128 on 2048 19.0 / 16.0, on up to 2048 14.9 / 15.1, on up to 2560 16.5 / 18.2; 64 x
+  // 8 of 14 / 2 of 64 on up to 2048 17.5 / 14.4.  Many rows: 256 of 32 / 8 of 128 on
+  // 1024 30.6 / 25.5, on 1280 29.1 / 30.3; 4 x 128 of 14 / 2 of 64 on 1024 20.4 / 19.7.
+  const int wide = D * p.nt;
   const bool every_cu = p.nt != 0 && (int64_t)B * Hk * p.row_tiles >= cus;
-  const int64_t enough = p.nt == 0 ? 1024 : (every_cu ? 2048 : 512);
+  const int64_t enough = p.nt == 0   ? 1024
+                         : every_cu  ? 2048
+                         : wide > 128 ? 640
+                         : wide > 64  ? 1024
+                                      : 1408;
   p.target = resident < 1 || capacity <= enough ? 1 : (int)resident;
   p.slots = p.target > 1 ? std::max(p.target, (p.target + 1) / 2 + B) : B;   // fa::find_chunk
   // (no more than the units that the table holds)
@@ -415,7 +423,7 @@ int fa_paged_read(const fa_paged_cache *cache, const int32_t *table, int64_t tab
 
 size_t fa_paged_attn_workspace_bytes(int B, int Sq, int H, int Hk, int D) {
   if (check_attn_sizes(B, Sq, H, Hk, D, FA_DTYPE_F16) != FA_OK) return 0;
-  return attn_plan(B, Sq, H, Hk, stream_cus(nullptr), INT64_MAX).bytes(B, Hk, D);
+  return attn_plan(B, Sq, H, Hk, D, stream_cus(nullptr), INT64_MAX).bytes(B, Hk, D);
 }
 
 int fa_paged_attn(const void *q, const fa_paged_cache *cache, const int32_t *table,
@@ -433,13 +441,13 @@ int fa_paged_attn(const void *q, const fa_paged_cache *cache, const int32_t *tab
   const int Hk = cache->heads;
   // (the size does not depend on the cache: a small one may leave it unused)
   const int cus = stream_cus(st);
-  const AttnPlan most = attn_plan(B, Sq, H, Hk, cus, INT64_MAX);
+  const AttnPlan most = attn_plan(B, Sq, H, Hk, D, cus, INT64_MAX);
   if ((int64_t)most.slots * Hk > kMaxThreads / 256) return FA_ERR_TOO_LARGE;
   if (most.bytes(B, Hk, D) > 0) {
     if (workspace == nullptr || workspace_bytes < most.bytes(B, Hk, D)) return FA_ERR_WORKSPACE;
     if (!aligned(workspace, 16)) return FA_ERR_ALIGNMENT;
   }
-  const AttnPlan p = attn_plan(B, Sq, H, Hk, cus, (int64_t)cache->width * cache->page_size);
+  const AttnPlan p = attn_plan(B, Sq, H, Hk, D, cus, (int64_t)cache->width * cache->page_size);
   fa::PagedAttnArgs a{};
   a.cache = device_cache(cache, table, table_stride);
   a.q = static_cast<const f16 *>(q);
