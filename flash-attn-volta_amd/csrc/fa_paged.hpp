@@ -340,7 +340,8 @@ __device__ __forceinline__ int scalar_load(const int32_t *p) {
 }
 
 // Has these kernel arguments in registers at this point: they are loaded together,
-// where the compiler would load each before its first use and wait for it there.
+// where the compiler would load each before its first use and wait for it there (one
+// query on 4096 tokens, two kernels: 8.45 / 8.25 us).
 template <typename T> __device__ __forceinline__ void have_one(T x) { asm volatile("" : : "s"(x)); }
 template <typename... T> __device__ __forceinline__ void have(T... x) { (have_one(x), ...); }
 
@@ -1084,7 +1085,7 @@ __global__ __launch_bounds__(256, 2) void fa_paged_rows_kernel(PagedAttnArgs a) 
 // Joins the chunks of each row of head blockIdx.y of sequence blockIdx.z (rows
 // whose sequence is one chunk were written by its workgroup): D / 4 lanes take 4
 // columns each of every NS-th chunk of a row, NS such groups a row.  Bound by
-// latency (NS = 8, few rows: 3.9 us) or by reading the chunks' rows (NS = 1: 8
+// latency (NS = 8, few rows: 3.8 us) or by reading the chunks' rows (NS = 1: 8
 // chunks of 8192 rows of 128, 6.9 us, 4.9 TB/s).
 template <typename E, int D, int NS, bool ONE>
 __global__ __launch_bounds__(256) void fa_paged_merge_kernel(PagedAttnArgs a) {
