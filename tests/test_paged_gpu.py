@@ -733,3 +733,27 @@ def test_a_batch_of_over_2_32_keys_that_may_be_split():
                            _i32(counts))
         assert torch.equal(out[at], alone[0])
         assert not out[[i for i in range(B) if i != at]].any()
+
+
+@pytest.mark.parametrize("B,Sq", [(1, 1), (5, 3), (70, 1), (3, 100)])
+def test_replays_split_as_their_lengths_say(B, Sq):
+    """One captured call serves batches of any lengths: many chunks, one, none."""
+    from flash_attn_volta import attend_paged
+    most = 2600
+    cache, table, model = _filled(B, [most] * B, 2, 64, 16, F16, 4, width=170)
+    q, t, lengths = _rand((B, Sq, 4, 64), F16, 8).cuda(), _i32(table), _i32([most] * B)
+    attend_paged(q, cache, t, lengths)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, lse = attend_paged(q, cache, t, lengths, return_softmax_lse=True)
+    rng = np.random.default_rng(B)
+    for now in ([0] * B, [most] * B, [most] + [1] * (B - 1), rng.integers(0, 200, B),
+                rng.integers(0, most, B), [100] * B):
+        lengths.copy_(_i32(now))
+        want, want_lse = attend_paged(q, cache, t, lengths, return_softmax_lse=True)
+        out.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(lse, want_lse)
+    _check_attend(out, lse, q, model, table, [100] * B)
